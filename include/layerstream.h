@@ -254,6 +254,80 @@ int ls_batch_profile(const LsBatch *b, LsBatchProfile *out);
  * it uses the NCCL all-reduce or the batch is not tensor-parallel. */
 int ls_batch_tp_peer(const LsBatch *b, int *on);
 
+/* ---- a paged K/V cache whose sequences share pages ------------------------------------------- */
+
+/* No counterpart in the reference. The page bookkeeping of a K/V cache over page pools in device
+ * memory that the caller owns, for `seqs` sequences, and the attention that reads it: sequences that
+ * were forked from one another (best-of-n sampling, many questions about one document) hold their
+ * common prefix in the same pages, a page is copied when a row is about to be written into one that
+ * others hold too, and attention reads a prefix that several sequences share once for all of them.
+ *
+ * Pools: k_pool, v_pool [layers][kv_heads][num_pages][page][hd], 16-bit (dtype), 16-byte aligned, on
+ * `device`; rows past a sequence's length are never used. page: a power of two in 8..65536; hd: 64 or
+ * 128. max_ctx: positions of one sequence; max_rows: largest seqs x M of a step (sizes the workspaces,
+ * which the cache owns and allocates here). device -1: the bookkeeping alone, without a GPU (pools
+ * NULL; attention is refused).
+ *
+ * A step, per decode or verify pass: ls_kv_begin gives every sequence s counts[s] (0..M) rows behind
+ * its length: pages are taken (the lowest free ones), shared pages among those that will be written are copied in
+ * every layer, and the pass's plan is laid out; ls_kv_attention once per layer; ls_kv_end keeps the
+ * first keep[s] of the rows (NULL: all) and returns the pages past them. A step that was begun and not
+ * ended is dropped by the next begin, and by any call that changes a table.
+ *
+ * Calls on one cache come from one thread at a time, and their GPU work, on whichever streams, must
+ * not overlap (the caller orders the streams). ls_kv_begin and ls_kv_compact are refused on a stream
+ * that is being captured; ls_kv_attention may be captured, and a replay runs the plan of the step that is
+ * begun then: it is valid between ls_kv_begin and ls_kv_end of a step with the M it was captured at,
+ * over the same qkv, rope and out buffers. Replays on one cache must not overlap either. */
+typedef struct LsKv LsKv;
+#define LS_KV_F16 0
+#define LS_KV_BF16 1
+
+typedef struct LsKvInfo {
+  uint64_t seqs, max_pages, num_pages; /* max_pages: page-table entries of one sequence */
+  uint64_t pages_used, pages_shared;   /* held by some sequence / by more than one */
+  uint64_t shared_positions;           /* positions the begun step reads once for several sequences */
+} LsKvInfo;
+
+int ls_kv_open(int device, uint64_t layers, uint64_t heads, uint64_t kv_heads, uint64_t hd, int dtype, uint64_t page,
+               uint64_t num_pages, uint64_t seqs, uint64_t max_ctx, uint64_t max_rows, void *k_pool, void *v_pool, LsKv **out);
+/* Waits for the device's work, then frees the workspaces (the pools stay the caller's). */
+int ls_kv_free(LsKv *kv);
+int ls_kv_info(const LsKv *kv, LsKvInfo *out);
+int ls_kv_len(const LsKv *kv, uint64_t seq, uint64_t *n);
+/* tables: [seqs][max_pages] page ids, -1 past each sequence's pages. */
+int ls_kv_tables(const LsKv *kv, int32_t *tables);
+/* Sequence seq holds exactly these pages (pages already held by others become shared), the first n
+ * positions of them cached; pages beyond those n need are kept for its next rows. */
+int ls_kv_set(LsKv *kv, uint64_t seq, const int32_t *pages, uint64_t npages, uint64_t n);
+/* Every dst[i] holds the first n positions of src, in the same pages; what it held is returned. */
+int ls_kv_fork(LsKv *kv, uint64_t src, const uint64_t *dst, uint64_t ndst, uint64_t n);
+int ls_kv_truncate(LsKv *kv, uint64_t seq, uint64_t n);
+/* Moves the pages in use to the lowest ids of the pools (in every layer, in stream order) and renames
+ * them in the tables, so that the pools' tail is free. *moved (optional): pages moved. */
+int ls_kv_compact(LsKv *kv, void *stream, uint64_t *moved);
+int ls_kv_begin(LsKv *kv, const uint32_t *counts, uint64_t M, void *stream);
+/* Causal grouped-query attention of the step's rows in layer `layer` (src/model.rs:261-282 over many
+ * sequences): row t of sequence s is row s * M + t of qkv (q | k | v: (heads + 2 kv_heads) * hd elements
+ * of the cache's type, rows qkv_stride elements apart, 0 = packed) and of out (heads * hd, out_stride).
+ * rope: f32 (cos, sin) pairs [position][hd / 2] by which q and k are rotated (rotate-half), or NULL when
+ * they are rotated already. k and v are rounded into the sequence's pages at position len + t; the row
+ * attends to positions 0 .. len + t. Rows t >= counts[s] are neither read nor written. Scores, softmax
+ * statistics and sums are f32; q (rotated) and the softmax weights are rounded to the cache's type for
+ * the tensor cores. Device pointers, 16-byte aligned; strides multiples of 8. An error that the kernels
+ * report (LS_ERR_DEVICE) comes with the next call. */
+int ls_kv_attention(LsKv *kv, uint64_t layer, const void *qkv, uint64_t qkv_stride, const float *rope, void *out,
+                    uint64_t out_stride, void *stream);
+int ls_kv_end(LsKv *kv, const uint32_t *keep);
+/* LS_ERR_ARG unless the page counts agree with the tables and the begun step's plan covers every row's
+ * positions exactly once (for tests; host work alone). */
+int ls_kv_self_check(const LsKv *kv);
+/* Copies rows [0, rows[i]) (NULL: whole pages) of page src[i] to page dst[i] in every layer and kv head of both
+ * pools, for pools as above of any head size that is a multiple of 8. src, dst, rows: host memory. No page may be
+ * written twice, or both read and written. */
+int ls_kv_copy_pages(void *k_pool, void *v_pool, uint64_t layers, uint64_t kv_heads, uint64_t hd, uint64_t page,
+                     uint64_t num_pages, const int32_t *src, const int32_t *dst, const int32_t *rows, uint64_t n, void *stream);
+
 /* ---- kernel-level entry points (microbenchmarks and parity tests) ---------------------------- */
 
 /* y[t][r] = dot(stored row r, x[t]) for t < M, with W given as `rows` stored rows in the .lsq

@@ -62,6 +62,13 @@ class SpecStats(C.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+KV_DTYPES = {"f16": 0, "bf16": 1}
+
+
+class KvInfo(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("seqs", "max_pages", "num_pages", "pages_used", "pages_shared", "shared_positions")]
+
+
 _lib = None
 
 # C signatures of include/layerstream.h
@@ -112,6 +119,20 @@ _SIGS = {
     "ls_batch_profile_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "ls_batch_profile": (C.c_int, [C.c_void_p, C.POINTER(BatchProfile)]),
     "ls_batch_tp_peer": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
+    "ls_kv_open": (C.c_int, [C.c_int] + [C.c_uint64] * 4 + [C.c_int] + [C.c_uint64] * 5 + [C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "ls_kv_free": (C.c_int, [C.c_void_p]),
+    "ls_kv_info": (C.c_int, [C.c_void_p, C.POINTER(KvInfo)]),
+    "ls_kv_len": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(C.c_uint64)]),
+    "ls_kv_tables": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "ls_kv_set": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64]),
+    "ls_kv_fork": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64]),
+    "ls_kv_truncate": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64]),
+    "ls_kv_compact": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64)]),
+    "ls_kv_begin": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "ls_kv_attention": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "ls_kv_end": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "ls_kv_self_check": (C.c_int, [C.c_void_p]),
+    "ls_kv_copy_pages": (C.c_int, [C.c_void_p, C.c_void_p] + [C.c_uint64] * 5 + [C.c_void_p] * 3 + [C.c_uint64, C.c_void_p]),
     "ls_attention_host": (C.c_int, [C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_uint64, C.c_uint64, C.c_void_p,
                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_double)]),
     "ls_batch_inject_error": (C.c_int, [C.c_void_p, C.c_int]),
@@ -537,6 +558,104 @@ def attention_paged(heads: int, kv_heads: int, hd: int, pos0: int, qkv: np.ndarr
     _check(lib().ls_attention_paged_host(heads, kv_heads, hd, rope_theta, pos0, M, _p(q), _p(k_pool), _p(v_pool), num_pages, page,
                                          _p(t), _p(out), iters, C.byref(ms)))
     return out, ms.value
+
+
+class KvCache:
+    """A paged K/V cache whose sequences share pages, over pools in device memory that the caller owns
+    (k_ptr, v_ptr: [layers][kv_heads][num_pages][page][hd], 16-bit). Sequences are forked, truncated and
+    compacted; a step is ``begin`` (rows per sequence), ``attention`` once per layer, ``end``. Attention
+    reads a prefix that several sequences hold in the same pages once for all of them.
+
+    The calls' GPU work must not overlap on one cache; see include/layerstream.h for capture.
+    device=-1 keeps the page tables alone, without a GPU."""
+
+    def __init__(self, k_ptr: int, v_ptr: int, layers: int, heads: int, kv_heads: int, hd: int, page: int, num_pages: int, seqs: int,
+                 max_ctx: int, max_rows: int, dtype: str = "f16", device: int = 0):
+        h = C.c_void_p()
+        _check(lib().ls_kv_open(device, layers, heads, kv_heads, hd, KV_DTYPES[dtype], page, num_pages, seqs, max_ctx, max_rows,
+                                k_ptr or None, v_ptr or None, C.byref(h)))
+        self._h, self.seqs = h, seqs
+        self.max_pages = self.info.max_pages
+
+    @property
+    def info(self) -> KvInfo:
+        i = KvInfo()
+        _check(lib().ls_kv_info(self._h, C.byref(i)))
+        return i
+
+    def length(self, seq: int) -> int:
+        n = C.c_uint64()
+        _check(lib().ls_kv_len(self._h, seq, C.byref(n)))
+        return n.value
+
+    def tables(self) -> np.ndarray:
+        """[seqs, max_pages] page ids, -1 past each sequence's pages."""
+        t = np.empty((self.seqs, self.max_pages), np.int32)
+        _check(lib().ls_kv_tables(self._h, _p(t)))
+        return t
+
+    def set_table(self, seq: int, pages, n: int):
+        """Sequence seq holds exactly these pages, n positions of them cached."""
+        p = np.ascontiguousarray(pages, np.int32)
+        _check(lib().ls_kv_set(self._h, seq, _p(p), p.size, n))
+
+    def fork(self, src: int, dst, n: int | None = None):
+        """dst (one sequence or several) hold the first n positions of src (None: all), in the same pages."""
+        d = np.array([dst] if isinstance(dst, (int, np.integer)) else list(dst), np.uint64)
+        _check(lib().ls_kv_fork(self._h, src, _p(d), d.size, self.length(src) if n is None else n))
+
+    def truncate(self, seq: int, n: int):
+        _check(lib().ls_kv_truncate(self._h, seq, n))
+
+    def compact(self, stream: int = 0) -> int:
+        """Moves the pages in use to the lowest ids; returns how many moved."""
+        m = C.c_uint64()
+        _check(lib().ls_kv_compact(self._h, stream, C.byref(m)))
+        return m.value
+
+    def begin(self, counts, M: int, stream: int = 0):
+        """A step: sequence s gets counts[s] (0..M) rows behind its length."""
+        _check(lib().ls_kv_begin(self._h, _p(self._per_seq(counts)), M, stream))
+
+    def attention(self, layer: int, qkv_ptr: int, out_ptr: int, rope_ptr: int = 0, qkv_stride: int = 0, out_stride: int = 0,
+                  stream: int = 0):
+        """The step's rows through one layer: row t of sequence s is row s * M + t of qkv and out."""
+        _check(lib().ls_kv_attention(self._h, layer, qkv_ptr, qkv_stride, rope_ptr, out_ptr, out_stride, stream))
+
+    def end(self, keep=None):
+        """Keeps the first keep[s] rows of the step (None: all)."""
+        _check(lib().ls_kv_end(self._h, None if keep is None else _p(self._per_seq(keep))))
+
+    def self_check(self):
+        _check(lib().ls_kv_self_check(self._h))
+
+    def _per_seq(self, a) -> np.ndarray:
+        a = np.array(a, np.int64)
+        if a.shape != (self.seqs,) or (a < 0).any() or (a > 0xFFFFFFFF).any():
+            raise ValueError(f"expected {self.seqs} counts")
+        return a.astype(np.uint32)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().ls_kv_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def kv_copy_pages(k_ptr: int, v_ptr: int, layers: int, kv_heads: int, hd: int, page: int, num_pages: int, src, dst, rows=None,
+                  stream: int = 0):
+    """Rows [0, rows[i]) (None: whole pages) of page src[i] to page dst[i], in every layer and kv head of both pools."""
+    s, d = np.array(src, np.int32), np.array(dst, np.int32)
+    r = None if rows is None else np.array(rows, np.int32)
+    if s.ndim != 1 or s.shape != d.shape or (r is not None and r.shape != s.shape):
+        raise ValueError("src, dst and rows must have the same length")
+    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, _p(s), _p(d), None if r is None else _p(r), s.size,
+                                  stream))
 
 
 def qgemv_rows_noalloc(bits: int, group: int, rows_ptr: int, rows: int, cols: int, x_ptr: int, M: int, y_ptr: int,

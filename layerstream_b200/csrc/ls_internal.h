@@ -460,6 +460,29 @@ struct NcclApi {
 const NcclApi& nccl_api();  // throws when libnccl.so.2 cannot be loaded
 void nccl_check(ncclResult_t r, const char* what);
 
+// ---- paged K/V cache over the caller's pools (ls_kv_cache.cpp): the calls behind ls_kv_* ----
+}  // namespace ls
+struct LsKv;
+struct LsKvInfo;
+namespace ls {
+LsKv* kv_open(int device, uint64_t layers, uint64_t heads, uint64_t kv_heads, uint64_t hd, int dtype, uint64_t page, uint64_t num_pages,
+              uint64_t seqs, uint64_t max_ctx, uint64_t max_rows, void* k_pool, void* v_pool);
+void kv_free(LsKv* kv);
+void kv_set(LsKv* kv, uint64_t s, const int32_t* pages, uint64_t npages, uint64_t n);
+void kv_fork(LsKv* kv, uint64_t src, const uint64_t* dst, uint64_t ndst, uint64_t n);
+void kv_truncate(LsKv* kv, uint64_t s, uint64_t n);
+uint64_t kv_compact(LsKv* kv, cudaStream_t st);
+void kv_begin(LsKv* kv, const uint32_t* counts, uint64_t M, cudaStream_t st);
+void kv_attention(LsKv* kv, uint64_t layer, const void* qkv, uint64_t qkv_stride, const float* rope, void* out, uint64_t out_stride,
+                  cudaStream_t st);
+void kv_end(LsKv* kv, const uint32_t* keep);
+void kv_self_check(const LsKv* kv);
+void kv_info(const LsKv* kv, LsKvInfo* out);
+uint64_t kv_len(const LsKv* kv, uint64_t s);
+void kv_tables(const LsKv* kv, int32_t* out);
+void kv_copy_pages(void* k, void* v, uint64_t layers, uint64_t kv_heads, uint64_t hd, uint64_t page, uint64_t num_pages, const int32_t* src,
+                   const int32_t* dst, const int32_t* rows, uint64_t n, cudaStream_t st);
+
 // ---- allocation-free GEMV (ls_noalloc.cu) ----
 void qgemv_rows_noalloc(int bits, int group, const uint8_t* rows_dev, uint64_t rows, uint64_t cols, const float* x_dev,
                         uint64_t M, float* y_dev, cudaStream_t s);

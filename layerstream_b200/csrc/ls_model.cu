@@ -2863,6 +2863,109 @@ int ls_qgemv_rows_noalloc(int bits, int group, const uint8_t* rows_dev, uint64_t
   return guard([&] { qgemv_rows_noalloc(bits, group, rows_dev, rows, cols, x_dev, M, y_dev, reinterpret_cast<cudaStream_t>(stream)); });
 }
 
+int ls_kv_open(int device, uint64_t layers, uint64_t heads, uint64_t kv_heads, uint64_t hd, int dtype, uint64_t page, uint64_t num_pages,
+               uint64_t seqs, uint64_t max_ctx, uint64_t max_rows, void* k_pool, void* v_pool, LsKv** out) {
+  return guard([&] {
+    NEED(out);
+    *out = nullptr;
+    *out = kv_open(device, layers, heads, kv_heads, hd, dtype, page, num_pages, seqs, max_ctx, max_rows, k_pool, v_pool);
+  });
+}
+
+int ls_kv_free(LsKv* kv) {
+  return guard([&] { kv_free(kv); });
+}
+
+int ls_kv_info(const LsKv* kv, LsKvInfo* out) {
+  return guard([&] {
+    NEED(kv);
+    NEED(out);
+    kv_info(kv, out);
+  });
+}
+
+int ls_kv_len(const LsKv* kv, uint64_t seq, uint64_t* n) {
+  return guard([&] {
+    NEED(kv);
+    NEED(n);
+    *n = kv_len(kv, seq);
+  });
+}
+
+int ls_kv_tables(const LsKv* kv, int32_t* tables) {
+  return guard([&] {
+    NEED(kv);
+    NEED(tables);
+    kv_tables(kv, tables);
+  });
+}
+
+int ls_kv_set(LsKv* kv, uint64_t seq, const int32_t* pages, uint64_t npages, uint64_t n) {
+  return guard([&] {
+    NEED(kv);
+    if (npages) NEED(pages);
+    kv_set(kv, seq, pages, npages, n);
+  });
+}
+
+int ls_kv_fork(LsKv* kv, uint64_t src, const uint64_t* dst, uint64_t ndst, uint64_t n) {
+  return guard([&] {
+    NEED(kv);
+    if (ndst) NEED(dst);
+    kv_fork(kv, src, dst, ndst, n);
+  });
+}
+
+int ls_kv_truncate(LsKv* kv, uint64_t seq, uint64_t n) {
+  return guard([&] {
+    NEED(kv);
+    kv_truncate(kv, seq, n);
+  });
+}
+
+int ls_kv_compact(LsKv* kv, void* stream, uint64_t* moved) {
+  return guard([&] {
+    NEED(kv);
+    const uint64_t n = kv_compact(kv, reinterpret_cast<cudaStream_t>(stream));
+    if (moved) *moved = n;
+  });
+}
+
+int ls_kv_begin(LsKv* kv, const uint32_t* counts, uint64_t M, void* stream) {
+  return guard([&] {
+    NEED(kv);
+    NEED(counts);
+    kv_begin(kv, counts, M, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int ls_kv_attention(LsKv* kv, uint64_t layer, const void* qkv, uint64_t qkv_stride, const float* rope, void* out, uint64_t out_stride,
+                    void* stream) {
+  return guard([&] {
+    NEED(kv);
+    kv_attention(kv, layer, qkv, qkv_stride, rope, out, out_stride, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int ls_kv_end(LsKv* kv, const uint32_t* keep) {
+  return guard([&] {
+    NEED(kv);
+    kv_end(kv, keep);
+  });
+}
+
+int ls_kv_self_check(const LsKv* kv) {
+  return guard([&] {
+    NEED(kv);
+    kv_self_check(kv);
+  });
+}
+
+int ls_kv_copy_pages(void* k_pool, void* v_pool, uint64_t layers, uint64_t kv_heads, uint64_t hd, uint64_t page, uint64_t num_pages,
+                     const int32_t* src, const int32_t* dst, const int32_t* rows, uint64_t n, void* stream) {
+  return guard([&] { kv_copy_pages(k_pool, v_pool, layers, kv_heads, hd, page, num_pages, src, dst, rows, n, reinterpret_cast<cudaStream_t>(stream)); });
+}
+
 int ls_batch_open(LsModel* m, uint64_t batch, uint64_t max_ctx, uint64_t max_block, LsBatch** out) {
   return guard([&] {
     NEED(m);
