@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "layerstream.h"
 #include "ls_device.cuh"
@@ -34,14 +35,16 @@
 namespace ls {
 
 constexpr int KV_THREADS = 352;  // 2 softmax warpgroups, 2 issuer warps, 1 producer warp
+constexpr int KV_SEGS_NEAR = 32;    // segments of a lane that are held in shared memory
 constexpr float KV_RESCALE = 8.0f;  // log2 growth of a row's maximum that O is rescaled for
 
 template <int HD>
 struct KvSmem {
-  static constexpr int kTile = 128 * HD * 2;      // Q tile, K chunk, V chunk
+  static constexpr int kTile = KV_TILE * HD * 2;    // Q tile
+  static constexpr int kChunk = KV_CHUNK * HD * 2;  // K chunk, V chunk
   static constexpr int kStages = HD == 64 ? 4 : 2;  // of K and of V, even: in the lanes' own phase lane t owns those of parity t
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile;
-  static constexpr int kTotal = kV + kStages * kTile + 1024;  // + alignment
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kChunk;
+  static constexpr int kTotal = kV + kStages * kChunk + 1024;  // + alignment
 };
 
 // ---- small device helpers -----------------------------------------------------------------------
@@ -50,6 +53,56 @@ __device__ __forceinline__ float kv_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t kv_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 kv_un2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t kv_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t kv_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float kv_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float kv_max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^z on the FMA units, for the share of the exponentials that the special-function units (16 a clock and SM)
+// would be late with: z = n + f, n the nearest integer (Cody and Waite's reduction; it sits in the low bits
+// of z + 1.5 * 2^23), 2^f by the quartic with the least largest relative error on [-1/2, 1/2] (Remez
+// exchange, 2.6e-6), n added to the exponent. z is clamped at -126, so the result is at least 2^-126 (ends
+// as zero or next to it in P); z up to 8 occurs. A NaN does not come through: the row's maximum carries it.
+__device__ __forceinline__ float2 kv_ex2_fma(uint64_t z) {
+  const float2 zf = kv_un2(z);
+  z = kv_f2(fmaxf(zf.x, -126.f), fmaxf(zf.y, -126.f));
+  const uint64_t r = kv_add2(z, kv_f2(12582912.f, 12582912.f));
+  const uint64_t f = kv_fma2(kv_add2(r, kv_f2(-12582912.f, -12582912.f)), kv_f2(-1.f, -1.f), z);
+  uint64_t p = kv_f2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+  p = kv_fma2(p, f, kv_f2(0x1.ca1444p-5f, 0x1.ca1444p-5f));
+  p = kv_fma2(p, f, kv_f2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = kv_fma2(p, f, kv_f2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = kv_fma2(p, f, kv_f2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  const float2 pf = kv_un2(p), rf = kv_un2(r);
+  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23)),
+                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23)));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
@@ -88,22 +141,72 @@ __device__ __forceinline__ void kv_ld32(uint32_t taddr, float* f) {
       : "r"(taddr)
       : "memory");
 }
+// Loads issued so far have landed; v (32 of their registers) is not read before.
+__device__ __forceinline__ void kv_wait32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]),
+                 "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]),
+                 "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+// Bounded wait on an mbarrier phase (a second or so), false and the CTA's abort flag on timeout. The loop is
+// not unrolled: it stands in the code two dozen times.
+__device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 22); i++) {
+    if (tc::mbar_try(bar, parity)) return true;
+    if ((i & 63) == 63 && *abort) return false;
+  }
+  *abort = 1;
+  return false;
+}
 __device__ __forceinline__ void kv_tma2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(tc::su32(bar))
       : "memory");
 }
-// Shared-memory matrix descriptor of a 128-byte-swizzled tile: 8-row groups 1024 bytes apart; lbo = bytes
-// between 64-element blocks of the contiguous dimension when that is the operand's M or N.
-__device__ __forceinline__ uint64_t kv_sdesc(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
-}
+// Low word of the shared-memory matrix descriptor of a 128-byte-swizzled tile (8-row groups 1024 bytes apart);
+// lbo = bytes between 64-element blocks of the contiguous dimension when that is the operand's M or N.
+__device__ __forceinline__ uint32_t kv_desc(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t KV_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // row-group stride, version 1, 128-byte swizzle
 // kind::f16, f32 accumulators, M = 128, N = n; b_mn: B's N dimension is the contiguous one.
 template <bool BF16>
 __host__ __device__ constexpr uint32_t kv_idesc(int n, bool b_mn) {
   return tc::idesc_f16(n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+// MMAs of a converged warp, issued by its elected lane (lead), so that their operands stay warp-uniform.
+__device__ __forceinline__ void kv_mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 x, {%2, %6};\n\t"
+      "mov.b64 y, {%3, %6};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%1], x, y, %4, p;\n\t}" ::"r"(lead),
+      "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(KV_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void kv_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%3, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], y, %4, p;\n\t}" ::"r"(lead),
+      "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(KV_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void kv_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(lead),
+      "r"(tc::su32(bar))
+      : "memory");
+}
+__device__ __forceinline__ uint32_t kv_elect() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void kv_st8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+               "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 
 // ---- the block's rows -----------------------------------------------------------------------------
@@ -155,6 +258,7 @@ __global__ void __launch_bounds__(256) kv_prep_kernel(const KvArgs a) {
   const int G = a.G, kvh = a.kv_heads, H = G * kvh, hd = a.hd, half = hd / 2, per = hd / 16;
   const int units = (H + 2 * kvh) * per;
   const int M = h.M;
+  pdl_wait();  // the rows; and the last call's kernels have read what is overwritten here
   const size_t total = (size_t)h.nseq * M * units;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
     const int row = (int)(i / units), u = (int)(i - (size_t)row * units);
@@ -211,27 +315,37 @@ __global__ void __launch_bounds__(256) kv_prep_kernel(const KvArgs a) {
 
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(KV_THREADS, 1)
-    kv_attn_kernel(const KvArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                   const __grid_constant__ CUtensorMap vmap) {
+    kv_attn_kernel(const KvArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qhalf,
+                   const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using SM = KvSmem<HD>;
   constexpr int NS = SM::kStages, CB = HD / 64;      // CB: 64-element column blocks of a row
-  constexpr uint32_t BLK = 128 * 128;                // bytes of one column block of a tile
-  constexpr uint32_t COL_O = 256;                    // tensor memory: S / P of lane t at 128 t, O at 256 + HD t
+  constexpr uint32_t QBLK = KV_TILE * 128, BLK = KV_CHUNK * 128;  // bytes of one column block of a Q tile, of a K or V chunk
+  // tensor memory: S of lane t at 128 t, O at 256 + HD t. P (two values a column): at hd 64 at 384 + 64 t; at hd 128,
+  // where nothing is left, over the upper half of S
+  constexpr bool OVER = HD == 128;
+  constexpr uint32_t COL_P = OVER ? 64 : 384, STEP_P = OVER ? 128 : 64, COL_O = 256;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS];
-  __shared__ uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2];
+  __shared__ uint64_t q_full[2][2], s_full[2], s_read[2], p_half[2], p_full[2], pv_done[2], o_free[2], turn;
+  __shared__ __align__(16) KvSeg s_segs[2][KV_SEGS_NEAR];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t smem = (tc::su32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem_gen = smem_raw + (smem - tc::su32(smem_raw));
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvProg pr = reinterpret_cast<const KvProg*>(a.plan + h.off_prog)[blockIdx.x];
   const KvSeg* const segs = reinterpret_cast<const KvSeg*>(a.plan + h.off_seg);
   pdl_trigger();
   if (pr.nseg[0] + pr.nseg[1] == 0) return;
 
+  constexpr int SEG16 = sizeof(KvSeg) / 16;
+  static_assert(sizeof(KvSeg) % 16 == 0, "segments are copied in 16-byte pieces");
+  for (int t = 0; t < 2; t++)
+    for (int i = tid; i < min(pr.nseg[t], KV_SEGS_NEAR) * SEG16; i += KV_THREADS)
+      reinterpret_cast<uint4*>(s_segs[t])[i] = reinterpret_cast<const uint4*>(segs + pr.seg[t])[i];
+  auto seg_of = [&](int t, int i) -> const KvSeg& { return i < KV_SEGS_NEAR ? s_segs[t][i] : segs[pr.seg[t] + i]; };
   if (tid == 0) {
     for (int s = 0; s < NS; s++) {
       tc::mbar_init(&k_full[s], 1);
@@ -240,12 +354,16 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       tc::mbar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; t++) {
-      tc::mbar_init(&q_full[t], 1);
+      tc::mbar_init(&q_full[t][0], 1);
+      tc::mbar_init(&q_full[t][1], 1);
       tc::mbar_init(&s_full[t], 1);
+      tc::mbar_init(&s_read[t], 4);
+      tc::mbar_init(&p_half[t], 4);
       tc::mbar_init(&p_full[t], 4);
       tc::mbar_init(&pv_done[t], 1);
       tc::mbar_init(&o_free[t], 4);
     }
+    tc::mbar_init(&turn, 4);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -263,14 +381,9 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   // phase in stage (2 j + t) % NS, so that each lane's own stages advance with that lane alone. Its
   // phase is the number of uses the stage had before.
   auto ring = [&](int chunk, int t, int& stage, uint32_t& phase) {
-    if (chunk < pr.pair_ch) {
-      stage = chunk % NS;
-      phase = (uint32_t)(chunk / NS);
-    } else {
-      const int v = 2 * (chunk - pr.pair_ch) + t;
-      stage = v % NS;
-      phase = (uint32_t)((pr.pair_ch - stage + NS - 1) / NS + v / NS);
-    }
+    const uint32_t pairs = pr.pair_ch, c = chunk, v = c < pairs ? c : 2 * (c - pairs) + t;
+    stage = v % NS;
+    phase = v / NS + (c < pairs ? 0 : (pairs + NS - 1 - stage) / NS);
   };
 
   if (warp == 10) {
@@ -279,14 +392,19 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     struct Cursor {
       int seg, end, j, chunk;
     };
-    Cursor cur[2] = {{pr.seg[0], pr.seg[0] + pr.nseg[0], 0, 0}, {pr.seg[1] + pr.npair, pr.seg[1] + pr.nseg[1], 0, pr.pair_ch}};
+    Cursor c = {0, pr.nseg[0], 0, 0}, other = {pr.npair, pr.nseg[1], 0, pr.pair_ch};  // of lane t, of the other lane
     bool ok = true;
     uint32_t issued = 0, parity = 0;  // per ring slot (K stages, then V stages): a copy was issued, its phase's parity
     int t = 0;
-    while (ok && (cur[0].seg < cur[0].end || cur[1].seg < cur[1].end)) {
-      if (cur[t].seg >= cur[t].end) t ^= 1;
-      Cursor& c = cur[t];
-      const KvSeg s = segs[c.seg];
+    auto swap = [&] {
+      const Cursor x = c;
+      c = other;
+      other = x;
+      t ^= 1;
+    };
+    while (ok && (c.seg < c.end || other.seg < other.end)) {
+      if (c.seg >= c.end) swap();
+      const KvSeg& s = seg_of(t, c.seg);
       const int pc = s.p0 + c.j * KV_CHUNK;
       const int npg = (min(KV_CHUNK, s.p1 - pc) + pg_rows - 1) / pg_rows;
       const int i = lane / CB, cb = lane - i * CB;
@@ -295,12 +413,12 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       int st;
       uint32_t ph;
       ring(c.chunk, t, st, ph);
-      const uint32_t off = (uint32_t)st * SM::kTile + cb * BLK + (uint32_t)(i * pg_rows) * 128u;
+      const uint32_t off = (uint32_t)st * SM::kChunk + cb * BLK + (uint32_t)(i * pg_rows) * 128u;
 #pragma unroll
       for (int kv = 0; kv < 2; kv++) {
         uint64_t* full = kv ? &v_full[st] : &k_full[st];
         uint64_t* empty = kv ? &v_empty[st] : &k_empty[st];
-        if (ph > 0) ok = ok && tc::mbar_wait_fast(empty, (ph - 1) & 1, &s_abort);
+        if (ph > 0) ok = ok && kv_wait(empty, (ph - 1) & 1, &s_abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) tc::mbar_expect_tx(full, (uint32_t)(npg * pg_rows) * HD * 2);
@@ -314,121 +432,203 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
         c.j = 0;
         c.seg++;
       }
-      if (c.chunk > pr.pair_ch || (c.chunk == pr.pair_ch && t == 0)) t = c.chunk == pr.pair_ch ? 0 : t ^ 1;
+      if (c.chunk > pr.pair_ch) swap();  // lane 0's pair chunks, then the lanes' own in turn
     }
     if (!ok) {  // copies in flight land before the CTA leaves
       int never = 0;
       for (int s = 0; s < 2 * NS; s++)
-        if (issued >> s & 1) (void)tc::mbar_wait(s < NS ? &k_full[s] : &v_full[s - NS], parity >> s & 1, &never);
+        if (issued >> s & 1) (void)kv_wait(s < NS ? &k_full[s] : &v_full[s - NS], parity >> s & 1, &never);
     }
   } else if (warp >= 8) {
-    // ---- MMA issuer of lane t ----
-    const int t = warp - 8;
-    if (lane == 0 && pr.nseg[t] > 0) {
+    // ---- MMA issuer of lane t (the whole warp runs it, one lane issues) ----
+    const int t = warp - 8, nseg = pr.nseg[t];
+    if (nseg > 0) {
+      const uint32_t lead = kv_elect();
       const uint32_t sq = smem + SM::kQ + t * SM::kTile;
-      const uint32_t t_s = tmem + t * 128, t_o = tmem + COL_O + t * HD;
-      auto load_q = [&](int seg) {
-        tc::mbar_expect_tx(&q_full[t], SM::kTile);
-        const int y = segs[seg].qrow;
-#pragma unroll
-        for (int cb = 0; cb < CB; cb++) kv_tma2d(sq + cb * BLK, &qmap, cb * 64, y, &q_full[t]);
+      const uint32_t t_s = tmem + t * 128, t_p = tmem + COL_P + t * STEP_P, t_o = tmem + COL_O + t * HD;
+      // Query tiles: segment i's may be loaded once the S products of the segment before it are done, or, when
+      // both are short and in different halves of the tile, those of the one before that (the MMA reads
+      // the other half's rows too, whatever they hold: no row's result depends on another row).
+      int loaded = 0;
+      auto load_ahead = [&](int i) {  // segments before i are done with their query tiles
+#pragma unroll 1
+        while (loaded < nseg && loaded <= i + 1) {
+          const KvSeg& s = seg_of(t, loaded);
+          const bool half = s.nrows <= KV_TILE / 2;
+          if (loaded == i + 1) {
+            const KvSeg& before = seg_of(t, i);
+            if (!half || before.nrows > KV_TILE / 2 || before.shift == s.shift) break;
+          }
+          uint64_t* bar = &q_full[t][loaded & 1];
+          if (lead) {
+            tc::mbar_expect_tx(bar, half ? SM::kTile / 2 : SM::kTile);
+#pragma unroll 1
+            for (int cb = 0; cb < CB; cb++) kv_tma2d(sq + cb * QBLK + s.shift * 128u, half ? &qhalf : &qmap, cb * 64, s.qrow, bar);
+          }
+          __syncwarp();
+          loaded++;
+        }
       };
-      load_q(pr.seg[t]);
-      int chunk = 0, nq = 1;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kv_wait(bar, parity, &s_abort)); };
+      auto cols = [&](const KvSeg& s, int j) { return min(KV_CHUNK, (s.p1 - s.p0 - j * KV_CHUNK + 31) & ~31); };
+      int si = 0, sj = 0, sc = 0;
+      // Chunk (i, j): round 0, its values of positions 64 .. 127 (P's upper half comes first); round 1, those of
+      // positions 0 .. 63; the next S, at hd 64 in round 1 ahead of them if its operands are there (a P V must
+      // not wait for the next chunk's copies, which may wait for the stage that it frees), else behind them in
+      // round 2. At hd 128, where P lies over S, it comes once the P V is done. Chunk -1 is round 2 alone.
+      int i = 0, j = 0;
       bool ok = true;
-      for (int i = 0; ok && i < pr.nseg[t]; i++) {
-        const int nch = segs[pr.seg[t] + i].nch;
-        for (int j = 0; j < nch; j++, chunk++) {
-          int st;
-          uint32_t ph;
+#pragma unroll 1
+      for (int chunk = -1; ok && (chunk < 0 || i < nseg); chunk++) {
+        bool done = si >= nseg;  // the next S has been issued, or there is none
+        int st = 0;
+        uint32_t ph = 0;
+        if (chunk >= 0) {
           ring(chunk, t, st, ph);
-          const bool pair = chunk < pr.pair_ch;
-          // scores: Q and the K chunk are in shared memory, the last P has been read
-          if (j == 0) ok = ok && tc::mbar_wait_fast(&q_full[t], i & 1, &s_abort);
-          ok = ok && tc::mbar_wait_fast(&k_full[st], ph & 1, &s_abort);
-          if (chunk > 0) ok = ok && tc::mbar_wait_fast(&pv_done[t], (chunk - 1) & 1, &s_abort);
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t sk = smem + SM::kK + st * SM::kTile;
-#pragma unroll
-          for (int k = 0; k < HD / 16; k++) {
-            const uint32_t o = (k / 4) * BLK + (k % 4) * 32u;
-            tc::mma_f16_ss(t_s, kv_sdesc(sq + o, 16), kv_sdesc(sk + o, 16), kv_idesc<BF16>(128, false), k > 0 ? 1u : 0u);
+          ok = wait(&v_full[st], ph & 1);
+          if (j == 0 && i > 0) ok = ok && wait(&o_free[t], (i - 1) & 1);
+        }
+#pragma unroll 1
+        for (int round = chunk < 0 ? 2 : 0; ok && round < 3; round++) {
+          if (round > 0 && !done) {
+            const KvSeg& s = seg_of(t, si);
+            int st_k;
+            uint32_t ph_k;
+            ring(sc, t, st_k, ph_k);
+            uint64_t* qb = &q_full[t][si & 1];
+            bool go = true;
+            if (round == 1) {
+              ok = wait(&s_read[t], chunk & 1);
+              if (sj == 0) load_ahead(si);
+              const bool q = !OVER && (sj > 0 || tc::mbar_poll(qb, (si >> 1) & 1));
+              go = __all_sync(0xffffffffu, q && tc::mbar_poll(&k_full[st_k], ph_k & 1));
+            } else {
+              if (sj == 0) load_ahead(si);
+              ok = (sj > 0 || wait(qb, (si >> 1) & 1)) && wait(&k_full[st_k], ph_k & 1);
+              if (OVER && chunk >= 0) ok = ok && wait(&pv_done[t], chunk & 1);
+            }
+            if (!ok) break;
+            if (go) {
+              tc::fence_after();
+              const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + st_k * SM::kChunk, 16);
+              const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(cols(s, sj) >> 3) << 17;
+#pragma unroll 1
+              for (int k = 0; k < HD / 16; k++)
+                kv_mma_ss(lead, t_s, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4), b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
+              kv_commit(lead, &s_full[t]);
+              kv_commit(lead, &k_empty[st_k]);
+              if (sc >= pr.pair_ch && lead) tc::mbar_arrive(&k_empty[st_k]);
+              __syncwarp();
+              done = true;
+              sc++;
+              if (++sj == s.nch) {
+                sj = 0;
+                si++;
+              }
+            }
           }
-          tc::commit(&s_full[t]);
-          tc::commit(&k_empty[st]);
-          if (!pair) tc::mbar_arrive(&k_empty[st]);
-          // values: P is in tensor memory (and S, hence Q and K, have been read)
-          ok = ok && tc::mbar_wait_fast(&p_full[t], chunk & 1, &s_abort);
-          if (ok && j == nch - 1 && i + 1 < pr.nseg[t]) {
-            load_q(pr.seg[t] + i + 1);
-            nq++;
+          if (round < 2) {
+            const KvSeg& s = seg_of(t, i);
+            const int ncol = cols(s, j);
+            ok = wait(round ? &p_full[t] : &p_half[t], chunk & 1);
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t b0 = kv_desc(smem + SM::kV + st * SM::kChunk, BLK);
+            const int k1 = round ? min(ncol, 64) >> 4 : ncol >> 4;
+            const bool first = j == 0 && (round == 0 || ncol <= 64);
+#pragma unroll 1
+            for (int k = round ? 0 : 4; k < k1; k++)
+              kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), !(first && (k & 3) == 0));
+            if (round == 1) {
+              kv_commit(lead, &pv_done[t]);
+              kv_commit(lead, &v_empty[st]);
+              if (chunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[st]);
+              __syncwarp();
+              if (++j == s.nch) {
+                j = 0;
+                i++;
+              }
+            }
           }
-          ok = ok && tc::mbar_wait_fast(&v_full[st], ph & 1, &s_abort);
-          if (j == 0 && i > 0) ok = ok && tc::mbar_wait_fast(&o_free[t], (i - 1) & 1, &s_abort);
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t sv = smem + SM::kV + st * SM::kTile;
-#pragma unroll
-          for (int k = 0; k < KV_CHUNK / 16; k++)
-            tc::mma_f16_ts(t_o, t_s + k * 8, kv_sdesc(sv + k * 2048u, BLK), kv_idesc<BF16>(HD, true), (j > 0 || k > 0) ? 1u : 0u);
-          tc::commit(&pv_done[t]);
-          tc::commit(&v_empty[st]);
-          if (!pair) tc::mbar_arrive(&v_empty[st]);
         }
       }
-      if (!ok) {  // the query tile in flight lands, the MMAs in flight end
+      if (!ok) {  // the query tiles in flight land, the MMAs in flight end
         int never = 0;
-        (void)tc::mbar_wait(&q_full[t], (nq - 1) & 1, &never);
-        tc::commit(&q_full[t]);
-        (void)tc::mbar_wait(&q_full[t], nq & 1, &never);
+        for (int i = max(0, loaded - 2); i < loaded; i++) (void)kv_wait(&q_full[t][i & 1], (i >> 1) & 1, &never);
+        uint64_t* bar = &q_full[t][loaded & 1];
+        kv_commit(lead, bar);
+        (void)kv_wait(bar, (loaded >> 1) & 1, &never);
       }
     }
   } else {
     // ---- softmax of lane t: one query row per thread ----
-    const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t t_s = tmem + ((uint32_t)(quad * 32) << 16) + t * 128;
-    const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + COL_O + t * HD;
+    const int t = warp >> 2, quad = warp & 3;
+    const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t t_s = at + t * 128, t_p = at + COL_P + t * STEP_P, t_o = at + COL_O + t * HD;
     const float cs = 1.4426950408889634f / sqrtf((float)HD);
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool done = __all_sync(0xffffffffu, kv_wait(bar, parity, &s_abort));
+      tc::fence_after();
+      return done;
+    };
+    auto arrive = [&](uint64_t* bar) {
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(bar);
+    };
     int chunk = 0;
     bool ok = true;
+#pragma unroll 1
     for (int i = 0; ok && i < pr.nseg[t]; i++) {
-      const KvSeg s = segs[pr.seg[t] + i];
-      const bool active = quad * 32 < s.nrows, row_ok = row < s.nrows;  // active: warp-uniform
+      const KvSeg& s = seg_of(t, i);
+      const int row = quad * 32 + lane - s.shift;
+      const bool row_ok = row >= 0 && row < s.nrows;
+      const bool active = quad * 32 >= s.shift && quad * 32 < s.shift + s.nrows;  // warp-uniform
       // last position the row sees
       int lim = s.p1 - 1;
       if (s.causal != INT_MAX && row_ok) lim = min(lim, s.causal + (s.trow0 + row) / a.G);
       float m_ref = -CUDART_INF_F, l = 0.f;
+#pragma unroll 1
       for (int j = 0; j < s.nch; j++, chunk++) {
         const int pc = s.p0 + j * KV_CHUNK;
-        ok = tc::mbar_wait_fast(&s_full[t], chunk & 1, &s_abort);
-        ok = __all_sync(0xffffffffu, ok);
+        const int ncol = min(KV_CHUNK, (s.p1 - pc + 31) & ~31);  // columns of S and P that the MMAs use
+        const int hi = ncol > 64;                                // the upper 64 are among them
+        ok = wait(&s_full[t], chunk & 1);
         if (!ok) break;
-        tc::fence_after();
-        if (active) {
-          float x[128];
-#pragma unroll
-          for (int q = 0; q < 4; q++) kv_ld32(t_s + q * 32, x + q * 32);
-          tc::wait_ld();
-          const int vis = lim - pc;  // columns 0 .. vis are visible
-          const bool all = __all_sync(0xffffffffu, vis >= KV_CHUNK - 1 || !row_ok);
+        // S, 64 columns at a time: both halves for the maximum, then the upper half's weights from registers and
+        // the lower half's from a second read. (Loops, not unrolled: the warps' roles together should stay
+        // within the instruction caches. With the whole row unrolled, 80 KB of code, the exponentials took 2000
+        // to 4000 cycles instead of 1500 whenever all SMs were busy.)
+        float x[64];
+        const int vis = lim - pc;  // columns 0 .. vis are visible
+        const bool all = __all_sync(0xffffffffu, vis >= KV_CHUNK - 1 || !row_ok);
+        auto load_s = [&](int h) {
+          kv_ld32(t_s + h * 64, x);
+          if (ncol > h * 64 + 32) kv_ld32(t_s + h * 64 + 32, x + 32);
+          kv_wait32(x);
+          kv_wait32(x + 32);
           if (!all) {
 #pragma unroll
-            for (int c = 0; c < 128; c++) x[c] = c <= vis ? x[c] : -CUDART_INF_F;
+            for (int c = 0; c < 64; c++) x[c] = h * 64 + c <= vis ? x[c] : -CUDART_INF_F;
           }
+        };
+        float mb = 0.f;
+        if (active) {
           float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll 1
+          for (int h = 0; h <= hi; h++) {
+            load_s(h);
 #pragma unroll
-          for (int c = 0; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-          const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cs;
+            for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = kv_max3_nan(mx[(c >> 1) & 3], x[c], x[c + 1]);
+          }
+          const float m_new = kv_max_nan(kv_max_nan(mx[0], mx[1]), kv_max_nan(mx[2], mx[3])) * cs;  // NaN if one score is
           if (j == 0) {
             m_ref = m_new;
-          } else if (__any_sync(0xffffffffu, row_ok && m_new > m_ref + KV_RESCALE)) {
+          } else if (__any_sync(0xffffffffu, row_ok && !(m_new <= m_ref + KV_RESCALE))) {
             // O and l to the new maximum, once the last P V has been added
-            ok = tc::mbar_wait_fast(&pv_done[t], (chunk - 1) & 1, &s_abort);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = wait(&pv_done[t], (chunk - 1) & 1);
             if (!ok) break;
-            tc::fence_after();
-            const float m2 = fmaxf(m_ref, m_new);
+            const float m2 = kv_max_nan(m_ref, m_new);
             const float f = m2 == -CUDART_INF_F ? 1.f : kv_ex2(m_ref - m2);
             m_ref = m2;
             l *= f;
@@ -442,38 +642,30 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
               tc::st16(t_o + q * 16, reinterpret_cast<uint32_t*>(o));
             }
           }
-          const float mb = m_ref == -CUDART_INF_F ? 0.f : m_ref;
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const float e0 = kv_ex2(fmaf(x[q * 32 + 2 * e], cs, -mb)), e1 = kv_ex2(fmaf(x[q * 32 + 2 * e + 1], cs, -mb));
-              ls[(2 * e) & 3] += e0;
-              ls[(2 * e + 1) & 3] += e1;
-              pk[e] = kv_pack<BF16>(e0, e1);
-            }
-            tc::st16(t_s + q * 16, pk);
+          // the exponents' base: 0 for a row that has seen nothing yet, NaN (and so the row's weights) for a
+          // maximum that is infinite or NaN
+          mb = m_ref == -CUDART_INF_F ? 0.f : m_ref + (m_ref - m_ref);
+          // lane 1 starts half a step behind: one lane's MMAs and waits then run under the other's exponentials
+          if (t == 1 && chunk == 0 && pr.pair_ch > 0) {
+            ok = wait(&turn, 0);
+            if (!ok) break;
           }
-          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-          tc::wait_st();
         }
         // V rows that nobody sees (past the range) are zeroed, and infinities and NaN of rows that
         // only some of the tile see; all four warps take part
-        const bool tail = pc + KV_CHUNK > s.p1;
+        const bool tail = pc + ncol > s.p1;
         const bool fresh = s.causal != INT_MAX && s.p1 > s.causal + 1 && pc + KV_CHUNK > s.causal + 1;
         if (tail || fresh) {
           int st;
           uint32_t ph;
           ring(chunk, t, st, ph);
-          ok = tc::mbar_wait_fast(&v_full[st], ph & 1, &s_abort);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = wait(&v_full[st], ph & 1);
           if (!ok) break;
-          uint8_t* sv = smem_gen + SM::kV + st * SM::kTile;
+          uint8_t* sv = smem_gen + SM::kV + st * SM::kChunk;
           const int r1 = min(KV_CHUNK, s.p1 - pc);
           const int r0 = fresh ? max(0, s.causal + 1 - pc) : r1;
-          for (int k = row; k < (KV_CHUNK - r0) * CB * 8; k += 128) {
+#pragma unroll 1
+          for (int k = quad * 32 + lane; k < (ncol - r0) * CB * 8; k += 128) {
             const int r = r0 + k / (CB * 8), c = k % (CB * 8);
             uint4* p = reinterpret_cast<uint4*>(sv + (c >> 3) * BLK + r * 128 + (c & 7) * 16);
             if (r >= r1) {
@@ -489,32 +681,65 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&p_full[t]);
+        // Before P is stored: the last P has been read. Warps without rows wait too, or their arrivals could count
+        // for the chunk before.
+        if (chunk > 0) {
+          ok = wait(&pv_done[t], (chunk - 1) & 1);
+          if (!ok) break;
+        }
+        const uint64_t cs2 = kv_f2(cs, cs), mb2 = kv_f2(-mb, -mb);
+        uint64_t ls[4] = {0, 0, 0, 0};
+#pragma unroll 1
+        for (int h = 1; h >= 0; h--) {
+          if (active && h < hi) load_s(h);
+          if (h == 0) arrive(&s_read[t]);  // at hd 64 the next S may take this one's place
+          if (active && h <= hi) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+              if (h * 64 + q * 32 >= ncol) continue;
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
+                float2 w;
+                if ((e & 7) == 1 || (e & 7) == 4 || (e & 7) == 6) {
+                  w = kv_ex2_fma(z);
+                } else {
+                  w = kv_un2(z);
+                  w.x = kv_ex2(w.x);
+                  w.y = kv_ex2(w.y);
+                }
+                ls[e & 3] = kv_add2(ls[e & 3], kv_f2(w.x, w.y));
+                pk[e] = kv_pack<BF16>(w.x, w.y);
+              }
+              tc::st16(t_p + h * 32 + q * 16, pk);
+            }
+            tc::wait_st();
+          }
+          if (h) arrive(&p_half[t]);
+        }
+        const float2 lf = kv_un2(kv_add2(kv_add2(ls[0], ls[1]), kv_add2(ls[2], ls[3])));
+        l += lf.x + lf.y;
+        arrive(&p_full[t]);
+        if (t == 0 && chunk == 0 && lane == 0) tc::mbar_arrive(&turn);
       }
       if (!ok) break;
-      ok = tc::mbar_wait_fast(&pv_done[t], (chunk - 1) & 1, &s_abort);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = wait(&pv_done[t], (chunk - 1) & 1);
       if (!ok) break;
-      tc::fence_after();
       if (active) {
         float* po = a.part + ((size_t)s.slot + row) * HD;
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < HD / 32; q++) {
           float o[32];
           kv_ld32(t_o + q * 32, o);
-          tc::wait_ld();
+          kv_wait32(o);
           if (row_ok)
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-              reinterpret_cast<float4*>(po + q * 32)[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; e++) kv_st8(po + q * 32 + 8 * e, o + 8 * e);
         }
         if (row_ok) reinterpret_cast<float2*>(a.part + (size_t)h.nslots * HD)[s.slot + row] = make_float2(m_ref, l);
       }
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&o_free[t]);
+      arrive(&o_free[t]);
     }
   }
 
@@ -532,96 +757,125 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
 
 // ---- the partials ---------------------------------------------------------------------------------
 
-// One warp per query row: the maxima of the row's partials, then their weighted sum in plan order
-// (the result does not depend on timing). BT: f16 in the batched GEMM's operand layout.
+// A query row's partials: their maximum, then their weighted sum, in plan order (the result does not
+// depend on timing). One warp per row, or, when the plan says that some row has many partials, the
+// block's four warps per row, each with every fourth of them. Bound by L2's latency when there are few rows
+// (sequence, units, then the maxima and four partials at once: three round trips), by its bandwidth
+// when there are many. BT: f16 in the batched GEMM's operand layout.
 template <int HD, bool BF16, bool BT>
 __global__ void __launch_bounds__(128) kv_merge_kernel(const KvArgs a) {
   constexpr int W = HD / 32;  // f32 per lane
+  using V = std::conditional_t<W == 4, float4, float2>;
+  __shared__ __align__(16) float s_acc[4][HD];
   pdl_trigger();
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvSeq* sqs = reinterpret_cast<const KvSeq*>(a.plan + h.off_seq);
-  const KvNode* nodes = reinterpret_cast<const KvNode*>(a.plan + h.off_node);
-  const int32_t* uoff = reinterpret_cast<const int32_t*>(a.plan + h.off_uoff);
-  const int32_t* useg = reinterpret_cast<const int32_t*>(a.plan + h.off_useg);
-  const int lane = threadIdx.x & 31;
-  const int G = a.G, kvh = a.kv_heads, H = G * kvh;
+  const KvUnit* units = reinterpret_cast<const KvUnit*>(a.plan + h.off_unit);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = a.G, kvh = a.kv_heads, H = G * kvh, M = h.M;
   const float2* pml = reinterpret_cast<const float2*>(a.part + (size_t)h.nslots * HD);
-  pdl_wait();
-  const size_t total = (size_t)h.nseq * h.M * H;
-  for (size_t it = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5); it < total; it += (size_t)gridDim.x * 4) {
-    const int orow = (int)(it / H), head = (int)(it - (size_t)orow * H);
-    const int s = orow / h.M, t = orow - s * h.M;
-    const KvSeq q = sqs[s];
+  const bool split = h.split_rows != 0;
+  const int ks = split ? 4 : 1, k0 = split ? warp : 0;
+  const int head0 = split ? blockIdx.y : blockIdx.y * 4 + warp, heads = split ? gridDim.y : gridDim.y * 4;
+  for (int orow = blockIdx.x; orow < h.nseq * M; orow += gridDim.x) {
+    const int s = orow / M, t = orow - s * M;
+    const KvSeq& q = sqs[s];
     if (t >= q.cnt) continue;
-    const int g = head / G, row = q.row0 + t * G + (head - g * G);
-    float m = -CUDART_INF_F, l = 0.f, acc[W];
+    for (int head = head0; head < H; head += heads) {
+      const int g = head / G, row = q.row0 + t * G + (head - g * G);
+      // the partials of the row's ranges: entries [0, c0), [c0, c1), [c1, n); entry i in partial row b + i * d
+      int b[KV_LEVELS], d[KV_LEVELS], c[KV_LEVELS], n = 0;
 #pragma unroll
-    for (int e = 0; e < W; e++) acc[e] = 0.f;
+      for (int l = 0; l < KV_LEVELS; l++) {
+        b[l] = d[l] = 0;
+        if (l < q.nlev) {
+          const int lr = row - q.lrow0[l];
+          const KvUnit u = units[q.lunit[l] + g * q.ltile[l] + lr / KV_TILE];
+          d[l] = u.nrows;
+          b[l] = u.base + lr % KV_TILE - n * u.nrows;
+          n += u.nseg;
+        }
+        c[l] = n;
+      }
+      auto slot_of = [&](int i) { return i < c[0] ? b[0] + i * d[0] : i < c[1] ? b[1] + i * d[1] : b[2] + i * d[2]; };
+      pdl_wait();
+      const float2 none = make_float2(-CUDART_INF_F, 0.f);
+      int slot = slot_of(lane);  // of the entry whose weight this lane holds
+      float2 ml = lane < n ? pml[slot] : none;
+      const int flag = t > 0 ? a.flags[s * kvh + g] : 0;
+      V v[4];
+      auto load = [&](int k) {  // entries k, k + ks, .. of the 32 whose slots the lanes hold
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int sl = __shfl_sync(0xffffffffu, slot, (k + e * ks) & 31);
+          if (k + e * ks < n) v[e] = *reinterpret_cast<const V*>(a.part + (size_t)sl * HD + lane * W);
+        }
+      };
+      load(k0);
+      float m = ml.x;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; pass++) {
+      for (int i = 32 + lane; i < n; i += 32) m = fmaxf(m, pml[slot_of(i)].x);
+      m = warp_max(m);
+      float l = 0.f, acc[W];
+#pragma unroll
+      for (int e = 0; e < W; e++) acc[e] = 0.f;
 #pragma unroll 1
-      for (int lv = 0; lv < q.nlev; lv++) {
-        const KvNode nd = nodes[q.node[lv]];
-        const int lr = row - nd.row0, u = nd.unit0 + g * nd.ntile + lr / KV_TILE;
-        const int k1 = uoff[u + 1];
-        for (int k0 = uoff[u]; k0 < k1; k0 += 32) {
-          int slot = 0;
-          float2 ml = make_float2(-CUDART_INF_F, 0.f);
-          if (k0 + lane < k1) {
-            slot = useg[k0 + lane] + lr % KV_TILE;
-            ml = __ldcg(pml + slot);
-          }
-          if (pass == 0) {
-            m = fmaxf(m, ml.x);
-            continue;
-          }
-          const float w = ml.x == -CUDART_INF_F ? 0.f : kv_ex2(ml.x - m);
-          l += w * ml.y;
-          const int n = min(32, k1 - k0);
-#pragma unroll 4
-          for (int k = 0; k < n; k++) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float* p = a.part + (size_t)__shfl_sync(0xffffffffu, slot, k) * HD + lane * W;
-            if constexpr (W == 4) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
-              acc[0] += wk * v.x;
-              acc[1] += wk * v.y;
-              acc[2] += wk * v.z;
-              acc[3] += wk * v.w;
-            } else {
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
-              acc[0] += wk * v.x;
-              acc[1] += wk * v.y;
+      for (int base = 0; base < n; base += 32) {
+        if (base > 0) {
+          slot = slot_of(base + lane);
+          ml = base + lane < n ? pml[slot] : none;
+        }
+        const float w = ml.x == -CUDART_INF_F ? 0.f : kv_ex2(ml.x - m);
+        l += w * ml.y;
+#pragma unroll 1
+        for (int k = base + k0; k < min(n, base + 32); k += 4 * ks) {
+          if (k > k0) load(k);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float wk = __shfl_sync(0xffffffffu, w, (k + e * ks) & 31);
+            if (k + e * ks < n) {
+              const float* f = reinterpret_cast<const float*>(&v[e]);
+#pragma unroll
+              for (int x = 0; x < W; x++) acc[x] += wk * f[x];
             }
           }
         }
       }
-      if (pass == 0) m = warp_max(m);
-    }
-    l = warp_sum(l);
-    const float inv = 1.0f / l;
+      l = warp_sum(l);
+      if (split) {
+        __syncthreads();  // (the last row's sums have been read)
+        *reinterpret_cast<V*>(&s_acc[warp][lane * W]) = *reinterpret_cast<V*>(acc);
+        __syncthreads();
+        if (warp != 0) continue;
 #pragma unroll
-    for (int e = 0; e < W; e++) acc[e] *= inv;
-    if (t > 0 && a.flags[s * kvh + g]) {  // infinities and NaN of the block's own V rows that this row sees
-      for (int tt = 1; tt <= t; tt++) {
-        const int pos = q.n + tt;
-        const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * W;
+        for (int x = 0; x < W; x++) acc[x] = (s_acc[0][lane * W + x] + s_acc[1][lane * W + x]) + (s_acc[2][lane * W + x] + s_acc[3][lane * W + x]);
+      }
+      const float inv = 1.0f / l;
 #pragma unroll
-        for (int e = 0; e < W; e += 2) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(a.v + src + e);
-          const uint32_t n = kv_nonfinite<BF16>(v);
-          const float2 f = kv_unpack<BF16>(v);
-          if (n & 0xffffu) acc[e] += f.x;
-          if (n >> 16) acc[e + 1] += f.y;
+      for (int e = 0; e < W; e++) acc[e] *= inv;
+      if (flag) {  // infinities and NaN of the block's own V rows that this row sees
+#pragma unroll 1
+        for (int tt = 1; tt <= t; tt++) {
+          const int pos = q.n + tt;
+          const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * W;
+#pragma unroll
+          for (int e = 0; e < W; e += 2) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(a.v + src + e);
+            const uint32_t nf = kv_nonfinite<BF16>(x);
+            const float2 f = kv_unpack<BF16>(x);
+            if (nf & 0xffffu) acc[e] += f.x;
+            if (nf >> 16) acc[e + 1] += f.y;
+          }
         }
       }
+      uint16_t* out = BT ? a.out + bt_off(orow, head * HD + lane * W, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * W;
+      if constexpr (W == 4)
+        *reinterpret_cast<uint2*>(out) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
+      else
+        *reinterpret_cast<uint32_t*>(out) = kv_pack<BF16>(acc[0], acc[1]);
     }
-    uint16_t* o = BT ? a.out + bt_off(orow, head * HD + lane * W, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * W;
-    if constexpr (W == 4)
-      *reinterpret_cast<uint2*>(o) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
-    else
-      *reinterpret_cast<uint32_t*>(o) = kv_pack<BF16>(acc[0], acc[1]);
   }
+  pdl_wait();  // (a warp without rows: the kernel after this one may rely on the one before it being done)
 }
 
 // ---- page copies ------------------------------------------------------------------------------------
@@ -731,6 +985,7 @@ void KvWork::open(const KvGeom& geom, bool is_bf16, int* err_word) {
   LS_CUDA(cudaMemset(q, 0, bq));
   LS_CUDA(cudaMemset(flags, 0, bf));
   kv_encode_map(&qmap, q, qrows, g.hd, KV_TILE, bf16);
+  kv_encode_map(&qmap_half, q, qrows, g.hd, KV_TILE / 2, bf16);
 }
 
 void KvWork::close() {
@@ -744,18 +999,18 @@ static void launch_kv_t(const KvWork& w, const KvAttn& a, const KvArgs& k, cudaS
   const size_t items = (size_t)a.rows * units;
   const int gp = (int)std::min<size_t>((items + 255) / 256, (size_t)w.g.nctas * 8);
   if (a.qkv_f32)
-    kv_prep_kernel<BF16, true><<<gp, 256, 0, s>>>(k);
+    launch_pdl(kv_prep_kernel<BF16, true>, dim3(gp), dim3(256), 0, s, k);
   else
-    kv_prep_kernel<BF16, false><<<gp, 256, 0, s>>>(k);
-  LS_CUDA(cudaGetLastError());
+    launch_pdl(kv_prep_kernel<BF16, false>, dim3(gp), dim3(256), 0, s, k);
   const size_t smem = KvSmem<HD>::kTotal;
   ensure_smem(kv_attn_kernel<HD, BF16>, smem);
-  launch_pdl(kv_attn_kernel<HD, BF16>, dim3(w.g.nctas), dim3(KV_THREADS), smem, s, k, w.qmap, *a.kmap, *a.vmap);
-  const int gm = (int)std::min<size_t>(((size_t)a.rows * w.g.heads + 3) / 4, (size_t)w.g.nctas * 16);
+  launch_pdl(kv_attn_kernel<HD, BF16>, dim3(w.g.nctas), dim3(KV_THREADS), smem, s, k, w.qmap, w.qmap_half, *a.kmap, *a.vmap);
+  // a block per row, the heads over grid.y as far as it takes to fill the GPU
+  const int gr = std::min(a.rows, w.g.nctas * 16), gh = std::min(w.g.heads, std::max((w.g.heads + 15) / 16, (w.g.nctas * 8 + gr - 1) / gr));
   if constexpr (!BF16) {
-    if (a.out_bt) return launch_pdl(kv_merge_kernel<HD, false, true>, dim3(gm), dim3(128), 0, s, k);
+    if (a.out_bt) return launch_pdl(kv_merge_kernel<HD, false, true>, dim3(gr, gh), dim3(128), 0, s, k);
   }
-  launch_pdl(kv_merge_kernel<HD, BF16, false>, dim3(gm), dim3(128), 0, s, k);
+  launch_pdl(kv_merge_kernel<HD, BF16, false>, dim3(gr, gh), dim3(128), 0, s, k);
 }
 
 void launch_kv_attention(const KvWork& w, const KvAttn& a, cudaStream_t s) {

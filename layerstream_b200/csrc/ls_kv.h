@@ -56,7 +56,9 @@ struct KvSeg {
   int32_t trow0;    // the tile's first row, counted from its sequence's first
   int32_t slot;     // partial row of the tile's first row
   int32_t flag;     // sequence * kv_heads + kv head (its own positions), -1 for a shared range
-  int32_t pad;
+  int32_t shift;    // tensor-memory lane of the tile's first row: 0, or 64 for every other short tile of a lane
+  int32_t unit;     // its unit
+  int32_t pad[3];
 };
 struct KvProg {  // one CTA's program
   int32_t seg[2];   // first segment of each lane
@@ -69,16 +71,18 @@ struct KvSeq {
   int32_t n, cnt;   // cached positions, rows of the block
   int32_t row0;     // first row in a kv head's query operand
   int32_t tab;      // offset of its page table
-  int32_t nlev;
-  int32_t node[KV_LEVELS];
+  int32_t nlev;     // nodes on its path; each one's first row, tiles, first unit:
+  int32_t lrow0[KV_LEVELS], ltile[KV_LEVELS], lunit[KV_LEVELS];  // unit of (kv head g, tile i) = lunit + g * ltile + i
+  int32_t pad[2];
 };
-struct KvNode {
-  int32_t row0, ntile, unit0, pad;  // unit of (kv head g, tile i) = unit0 + g * ntile + i
+struct KvUnit {     // a tile's partials: segment k's of its row r in partial row base + k * nrows + r
+  int32_t base, nseg, nrows, pad;
 };
 struct KvHdr {
   int32_t M, nseq, R, max_pages;  // R: rows of a kv head's query operand
-  int32_t off_prog, off_seg, off_seq, off_node, off_uoff, off_useg;  // byte offsets in the plan
-  int32_t nslots, pad;
+  int32_t off_prog, off_seg, off_seq, off_unit;  // byte offsets in the plan
+  int32_t nslots, split_rows;  // split_rows: some row has many partials (kv_merge_kernel)
+  int32_t pad[2];
 };
 
 struct KvGeom {
@@ -129,14 +133,16 @@ class KvPlanner {
   uint64_t version_ = ~0ull;
   size_t shared_pos_ = 0;
   std::vector<Node> nodes_;
-  std::vector<KvNode> dnodes_;
+  struct DNode {
+    int row0, ntile, unit0;
+  };
+  std::vector<DNode> dnodes_;
   std::vector<KvSeq> dseqs_;
   std::vector<Job> jobs_;
   std::vector<Piece> pieces_;
   std::vector<KvSeg> segs_, lane_[2];
   std::vector<KvProg> progs_;
-  std::vector<std::pair<int, int>> uslot_;  // (unit, slot) in order of creation
-  std::vector<int32_t> uoff_, useg_;
+  std::vector<KvUnit> units_;
   void tree(const std::vector<KvSeqIn>& seqs);
 };
 
@@ -150,7 +156,7 @@ struct KvWork {
   float* part = nullptr;       // O partials [slots][hd], then (m, l) [slots][2]
   int* flags = nullptr;        // [nseq * kv_heads]: a new V row holds an infinity or a NaN
   int* err = nullptr;          // device-visible error word (1: a bounded wait gave up)
-  CUtensorMap qmap{};
+  CUtensorMap qmap{}, qmap_half{};  // boxes of a tile's rows, of half a tile's
   void* mem = nullptr;         // the allocation behind plan, q, part and flags
   void open(const KvGeom& geom, bool is_bf16, int* err_word);  // on the current device
   void close();

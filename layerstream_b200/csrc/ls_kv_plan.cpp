@@ -12,14 +12,20 @@ namespace ls {
 // A range is read for its sequences at once when that saves at least this many position reads over
 // the sequences reading it one by one: below it, the extra partial that every row then leaves and
 // joins costs about as much as the reads.
-constexpr long long kMinSaved = 2 * KV_CHUNK;
+constexpr long long kMinSaved = 256;
+
+// Time of a CTA's work in units of one pair chunk: a chunk for two tiles, for one tile (the two lanes work on
+// different ones), and what a segment costs before its first chunk and after its last.
+constexpr double kPairChunk = 1.0, kSingleChunk = 0.7, kPairStart = 2.0, kSingleStart = 0.3;
+
+// A row with more partials than this is merged by four warps instead of one.
+constexpr int kSplitRows = 8;
 
 static size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t KvGeom::plan_cap() const {
   return align16(sizeof(KvHdr)) + align16(nctas * sizeof(KvProg)) + align16(segs_cap() * sizeof(KvSeg)) +
-         align16(nseq * sizeof(KvSeq)) + align16(2 * (size_t)nseq * sizeof(KvNode)) + align16((units_cap() + 1) * 4) +
-         align16(segs_cap() * 4);
+         align16(nseq * sizeof(KvSeq)) + align16(units_cap() * sizeof(KvUnit));
 }
 
 // Groups the sequences with rows by their first page, then each group by the page after its common
@@ -29,9 +35,14 @@ size_t KvGeom::plan_cap() const {
 void KvPlanner::tree(const std::vector<KvSeqIn>& seqs) {
   order_.clear();
   shared_.clear();
-  std::vector<int> act;
+  std::vector<int> act, alone;
   for (size_t i = 0; i < seqs.size(); i++)
-    if (seqs[i].cnt > 0) act.push_back((int)i);
+    if (seqs[i].cnt > 0) {
+      // rows that fill tiles of their own read the prefix once per pair of tiles either way: as one range with
+      // their own positions they leave one partial less
+      const int rows = seqs[i].cnt * g.G(), pairs = (rows + 2 * KV_TILE - 1) / (2 * KV_TILE);
+      (rows * 5 >= pairs * 2 * KV_TILE * 4 ? alone : act).push_back((int)i);
+    }
   auto full = [&](int i) { return seqs[i].n >> g.shift; };
   // runs of `ids` that agree on the page at depth d, in order of first appearance; sequences without a
   // full page there come last, one by one
@@ -81,6 +92,7 @@ void KvPlanner::tree(const std::vector<KvSeqIn>& seqs) {
     }
     if (base) shared_[at1].last = (int)order_.size();
   }
+  order_.insert(order_.end(), alone.begin(), alone.end());
 }
 
 void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version) {
@@ -112,14 +124,14 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
     shared_pos_ += nd.b - nd.a;
     for (int o = nd.first; o < nd.last; o++) {
       KvSeq& d = dseqs_[order_[o]];
-      d.node[d.nlev++] = (int)k;
+      d.lunit[d.nlev++] = (int)k;  // the node, until its unit is known
       from[order_[o]] = nd.b;
     }
   }
   for (size_t o = 0; o < order_.size(); o++) {
     const int i = order_[o];
     KvSeq& d = dseqs_[i];
-    d.node[d.nlev++] = (int)nodes_.size();
+    d.lunit[d.nlev++] = (int)nodes_.size();
     nodes_.push_back({from[i], seqs[i].n + seqs[i].cnt, (int)o, (int)o + 1, seqs[i].tab, true});
   }
   // units, jobs: pairs of tiles of one kv head first, then single tiles
@@ -138,9 +150,16 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   for (size_t k = 0; k < nodes_.size(); k++) {
     const auto [row0, nrows] = rows_of(nodes_[k]);
     const int nt = (nrows + KV_TILE - 1) / KV_TILE;
-    dnodes_.push_back({row0, nt, units, 0});
+    dnodes_.push_back({row0, nt, units});
     units += nt * kvh;
   }
+  for (int i : order_)
+    for (int l = 0; l < dseqs_[i].nlev; l++) {
+      const DNode& d = dnodes_[dseqs_[i].lunit[l]];
+      dseqs_[i].lrow0[l] = d.row0;
+      dseqs_[i].ltile[l] = d.ntile;
+      dseqs_[i].lunit[l] = d.unit0;
+    }
   for (int pass = 0; pass < 2; pass++)
     for (size_t k = 0; k < nodes_.size(); k++) {
       const auto [row0, nrows] = rows_of(nodes_[k]);
@@ -158,22 +177,22 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
         }
       }
     }
-  // the jobs' chunks in order, dealt to the CTAs in equal shares
-  const double cost_pair = 1.0, cost_single = 1.0;
+  // the jobs' chunks in order, dealt to the CTAs in equal shares of time
   double total = 0;
-  for (const Job& j : jobs_) total += j.nch * (j.ntiles == 2 ? cost_pair : cost_single);
+  for (const Job& j : jobs_) total += j.ntiles == 2 ? kPairStart + j.nch * kPairChunk : kSingleStart + j.nch * kSingleChunk;
   const double share = std::max(total / g.nctas, 1e-9);
   pieces_.clear();
   {
     int cta = 0;
-    double x = 0;  // cost dealt so far
+    double x = 0;  // time dealt so far
     for (size_t k = 0; k < jobs_.size(); k++) {
-      const double q = jobs_[k].ntiles == 2 ? cost_pair : cost_single;
+      const bool pair = jobs_[k].ntiles == 2;
+      const double q = pair ? kPairChunk : kSingleChunk, o = pair ? kPairStart : kSingleStart;
       int c = 0;
       while (c < jobs_[k].nch) {
         int take = jobs_[k].nch - c;
         if (cta < g.nctas - 1) {
-          const double room = share * (cta + 1) - x;
+          const double room = share * (cta + 1) - x - (c == 0 ? o : 0);
           const int fit = (int)(room / q + 0.5);
           if (fit < 1) {
             cta++;
@@ -182,7 +201,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
           take = std::min(take, fit);
         }
         pieces_.push_back({cta, (int)k, c, take});
-        x += take * q;
+        x += take * q + (c == 0 ? o : 0);
         c += take;
       }
     }
@@ -190,8 +209,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   // segments
   segs_.clear();
   progs_.assign(g.nctas, KvProg{});
-  uslot_.clear();
-  int slots = 0;
+  units_.assign(units, KvUnit{});
   auto emit = [&](std::vector<KvSeg>& to, const Job& j, int tile, int c0, int nch) {
     const Node& nd = nodes_[j.node];
     const auto [row0, nrows] = rows_of(nd);
@@ -205,10 +223,10 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
     s.nch = nch;
     s.causal = nd.own ? seqs[order_[nd.first]].n : INT_MAX;
     s.trow0 = tile * KV_TILE;
-    s.slot = slots;
     s.flag = nd.own ? order_[nd.first] * kvh + j.g : -1;
-    uslot_.push_back({dnodes_[j.node].unit0 + j.g * dnodes_[j.node].ntile + tile, slots});
-    slots += s.nrows;
+    s.unit = dnodes_[j.node].unit0 + j.g * dnodes_[j.node].ntile + tile;
+    s.slot = units_[s.unit].nseg++;  // which of the unit's segments, until its partials have a place
+    units_[s.unit].nrows = s.nrows;
     to.push_back(s);
   };
   for (size_t k = 0; k < pieces_.size();) {
@@ -234,20 +252,30 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
       if (p.nch > n0) emit(lane_[1], j, j.tile, p.c0 + n0, p.nch - n0);
       left0 -= n0;
     }
+    // short tiles of a lane's own phase alternate between the halves of its tensor-memory lanes (the other
+    // lane starts with the other half: their warps then sit on different schedulers)
+    for (int t = 0; t < 2; t++)
+      for (size_t i = pr.npair; i < lane_[t].size(); i++)
+        if (lane_[t][i].nrows <= KV_TILE / 2) lane_[t][i].shift = ((int)i - pr.npair + t) % 2 * (KV_TILE / 2);
     for (int t = 0; t < 2; t++) {
       pr.seg[t] = (int)segs_.size();
       pr.nseg[t] = (int)lane_[t].size();
       segs_.insert(segs_.end(), lane_[t].begin(), lane_[t].end());
     }
   }
-  uoff_.assign(units + 1, 0);
-  for (const auto& u : uslot_) uoff_[u.first + 1]++;
-  for (int u = 0; u < units; u++) uoff_[u + 1] += uoff_[u];
-  useg_.resize(uslot_.size());
-  {
-    std::vector<int32_t> at(uoff_.begin(), uoff_.end());
-    for (const auto& u : uslot_) useg_[at[u.first]++] = u.second;
+  int slots = 0, most = 0;  // most: partials of one row
+  for (KvUnit& u : units_) {
+    u.base = slots;
+    slots += u.nseg * u.nrows;
   }
+  for (KvSeg& s : segs_) s.slot = units_[s.unit].base + s.slot * s.nrows;
+  for (int i : order_)
+    for (int kh = 0; kh < kvh; kh++) {
+      int n = 0;
+      for (int l = 0; l < dseqs_[i].nlev; l++)
+        n += units_[dseqs_[i].lunit[l] + kh * dseqs_[i].ltile[l] + (dseqs_[i].row0 - dseqs_[i].lrow0[l]) / KV_TILE].nseg;
+      most = std::max(most, n);
+    }
   if ((size_t)R > g.rows_cap() || (size_t)units > g.units_cap() || segs_.size() > g.segs_cap() || (size_t)slots > g.slots_cap())
     LS_THROW(LS_ERR_ARG, "internal: an attention plan outgrew its workspace");
   // pack
@@ -257,6 +285,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   h.R = R;
   h.max_pages = g.max_pages;
   h.nslots = slots;
+  h.split_rows = most > kSplitRows;
   size_t at = align16(sizeof(KvHdr));
   auto place = [&](int32_t& off, size_t n) {
     off = (int32_t)at;
@@ -265,9 +294,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   place(h.off_prog, progs_.size() * sizeof(KvProg));
   place(h.off_seg, segs_.size() * sizeof(KvSeg));
   place(h.off_seq, dseqs_.size() * sizeof(KvSeq));
-  place(h.off_node, dnodes_.size() * sizeof(KvNode));
-  place(h.off_uoff, uoff_.size() * 4);
-  place(h.off_useg, useg_.size() * 4);
+  place(h.off_unit, units_.size() * sizeof(KvUnit));
   bytes.resize(at);
   auto put = [&](int32_t off, const void* p, size_t n) {
     if (n) std::memcpy(bytes.data() + off, p, n);
@@ -276,9 +303,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   put(h.off_prog, progs_.data(), progs_.size() * sizeof(KvProg));
   put(h.off_seg, segs_.data(), segs_.size() * sizeof(KvSeg));
   put(h.off_seq, dseqs_.data(), dseqs_.size() * sizeof(KvSeq));
-  put(h.off_node, dnodes_.data(), dnodes_.size() * sizeof(KvNode));
-  put(h.off_uoff, uoff_.data(), uoff_.size() * 4);
-  put(h.off_useg, useg_.data(), useg_.size() * 4);
+  put(h.off_unit, units_.data(), units_.size() * sizeof(KvUnit));
   if (at > g.plan_cap()) LS_THROW(LS_ERR_ARG, "internal: an attention plan outgrew its workspace");
 }
 
@@ -292,9 +317,7 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
   const auto* prog = reinterpret_cast<const KvProg*>(bytes.data() + h.off_prog);
   const auto* seg = reinterpret_cast<const KvSeg*>(bytes.data() + h.off_seg);
   const auto* sq = reinterpret_cast<const KvSeq*>(bytes.data() + h.off_seq);
-  const auto* nd = reinterpret_cast<const KvNode*>(bytes.data() + h.off_node);
-  const auto* uoff = reinterpret_cast<const int32_t*>(bytes.data() + h.off_uoff);
-  const auto* useg = reinterpret_cast<const int32_t*>(bytes.data() + h.off_useg);
+  const auto* unit = reinterpret_cast<const KvUnit*>(bytes.data() + h.off_unit);
   const int G = g.G();
   need((size_t)h.R <= g.rows_cap() && (size_t)h.nslots <= g.slots_cap() && h.nseq == (int)seqs.size(), "header");
   // every program's segments: in bounds, pairs aligned, slots written once
@@ -312,6 +335,7 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
         need(s.nrows >= 1 && s.nrows <= KV_TILE && s.kv_head >= 0 && s.kv_head < g.kv_heads, "rows");
         need(s.qrow >= s.kv_head * h.R && s.qrow + s.nrows <= (s.kv_head + 1) * h.R, "query rows");
         need(s.nch >= 1 && s.p0 >= 0 && s.p1 > s.p0 + (s.nch - 1) * KV_CHUNK && s.p1 <= s.p0 + s.nch * KV_CHUNK, "positions");
+        need(s.shift == 0 || (s.shift == KV_TILE / 2 && s.nrows <= KV_TILE / 2 && i >= p.npair), "lane half");
         need(s.p0 % std::min(g.page(), KV_CHUNK) == 0, "page alignment");
         need(s.slot >= 0 && s.slot + s.nrows <= h.nslots, "partial rows");
         for (int r = 0; r < s.nrows; r++) {
@@ -348,15 +372,15 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
           const int row = sq[i].row0 + t * G + j;
           std::vector<std::pair<int, int>> cover;
           for (int l = 0; l < sq[i].nlev; l++) {
-            const KvNode& n = nd[sq[i].node[l]];
-            const int lr = row - n.row0, tile = lr / KV_TILE;
-            need(lr >= 0 && tile < n.ntile, "tile");
-            const int u = n.unit0 + kh * n.ntile + tile;
-            need(uoff[u + 1] > uoff[u], "a unit without segments");
-            for (int k = uoff[u]; k < uoff[u + 1]; k++) {
-              auto it = at.find(useg[k]);
+            const int lr = row - sq[i].lrow0[l], tile = lr / KV_TILE;
+            need(lr >= 0 && tile < sq[i].ltile[l], "tile");
+            const KvUnit& u = unit[sq[i].lunit[l] + kh * sq[i].ltile[l] + tile];
+            need(u.nseg > 0, "a unit without segments");
+            for (int k = 0; k < u.nseg; k++) {
+              auto it = at.find(u.base + k * u.nrows);
               need(it != at.end(), "slot of a segment");
               const KvSeg& s = *it->second;
+              need(s.nrows == u.nrows, "rows of a unit");
               need(s.kv_head == kh && s.qrow + lr % KV_TILE == kh * h.R + row && lr % KV_TILE < s.nrows, "row of a segment");
               if (s.causal != INT_MAX) need(s.causal == seqs[i].n && (s.trow0 + lr % KV_TILE) / G == t && s.flag == i * g.kv_heads + kh, "causal limit");
               else need(s.p1 <= seqs[i].n, "a shared range ends inside the cached positions");
