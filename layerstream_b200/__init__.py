@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 
 import numpy as np
 
@@ -179,6 +180,11 @@ def _u32(a):
 
 def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _addr(a: np.ndarray) -> int:
+    """The array's address, without _p's cost (4 us); the caller keeps the array."""
+    return a.__array_interface__["data"][0]
 
 
 class Model:
@@ -591,18 +597,18 @@ class KvCache:
     def tables(self) -> np.ndarray:
         """[seqs, max_pages] page ids, -1 past each sequence's pages."""
         t = np.empty((self.seqs, self.max_pages), np.int32)
-        _check(lib().ls_kv_tables(self._h, _p(t)))
+        _check(lib().ls_kv_tables(self._h, _addr(t)))
         return t
 
     def set_table(self, seq: int, pages, n: int):
         """Sequence seq holds exactly these pages, n positions of them cached."""
         p = np.ascontiguousarray(pages, np.int32)
-        _check(lib().ls_kv_set(self._h, seq, _p(p), p.size, n))
+        _check(lib().ls_kv_set(self._h, seq, _addr(p), p.size, n))
 
     def fork(self, src: int, dst, n: int | None = None):
         """dst (one sequence or several) hold the first n positions of src (None: all), in the same pages."""
-        d = np.array([dst] if isinstance(dst, (int, np.integer)) else list(dst), np.uint64)
-        _check(lib().ls_kv_fork(self._h, src, _p(d), d.size, self.length(src) if n is None else n))
+        d = array("Q", [dst] if isinstance(dst, int) else dst)
+        _check(lib().ls_kv_fork(self._h, src, d.buffer_info()[0], len(d), self.length(src) if n is None else n))
 
     def truncate(self, seq: int, n: int):
         _check(lib().ls_kv_truncate(self._h, seq, n))
@@ -615,7 +621,8 @@ class KvCache:
 
     def begin(self, counts, M: int, stream: int = 0):
         """A step: sequence s gets counts[s] (0..M) rows behind its length."""
-        _check(lib().ls_kv_begin(self._h, _p(self._per_seq(counts)), M, stream))
+        c = self._per_seq(counts)
+        _check(lib().ls_kv_begin(self._h, c.buffer_info()[0], M, stream))
 
     def attention(self, layer: int, qkv_ptr: int, out_ptr: int, rope_ptr: int = 0, qkv_stride: int = 0, out_stride: int = 0,
                   stream: int = 0):
@@ -624,16 +631,20 @@ class KvCache:
 
     def end(self, keep=None):
         """Keeps the first keep[s] rows of the step (None: all)."""
-        _check(lib().ls_kv_end(self._h, None if keep is None else _p(self._per_seq(keep))))
+        k = None if keep is None else self._per_seq(keep)
+        _check(lib().ls_kv_end(self._h, k.buffer_info()[0] if k else None))
 
     def self_check(self):
         _check(lib().ls_kv_self_check(self._h))
 
-    def _per_seq(self, a) -> np.ndarray:
-        a = np.array(a, np.int64)
-        if a.shape != (self.seqs,) or (a < 0).any() or (a > 0xFFFFFFFF).any():
+    def _per_seq(self, a) -> array:
+        try:
+            c = array("I", a)
+        except OverflowError as e:
+            raise ValueError("counts must not be negative") from e
+        if len(c) != self.seqs:
             raise ValueError(f"expected {self.seqs} counts")
-        return a.astype(np.uint32)
+        return c
 
     def close(self):
         if getattr(self, "_h", None):
@@ -654,8 +665,8 @@ def kv_copy_pages(k_ptr: int, v_ptr: int, layers: int, kv_heads: int, hd: int, p
     r = None if rows is None else np.array(rows, np.int32)
     if s.ndim != 1 or s.shape != d.shape or (r is not None and r.shape != s.shape):
         raise ValueError("src, dst and rows must have the same length")
-    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, _p(s), _p(d), None if r is None else _p(r), s.size,
-                                  stream))
+    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, _addr(s), _addr(d), None if r is None else _addr(r),
+                                  s.size, stream))
 
 
 def qgemv_rows_noalloc(bits: int, group: int, rows_ptr: int, rows: int, cols: int, x_ptr: int, M: int, y_ptr: int,

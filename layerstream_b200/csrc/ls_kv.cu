@@ -880,14 +880,20 @@ __global__ void __launch_bounds__(128) kv_merge_kernel(const KvArgs a) {
 
 // ---- page copies ------------------------------------------------------------------------------------
 
-constexpr int KV_COPIES = 1024;  // copies of one launch (they travel in its parameters)
+// Copies of one launch (they travel in its parameters; few of them in a short list, since parameters cost the
+// host time), grouped in runs that share source and rows: a run reads its source once.
+constexpr int KV_COPIES = 1024, KV_FEW_COPIES = 64, KV_RUN = 8;
+template <int N>
 struct KvCopyList {
-  PageCopy c[KV_COPIES];
+  int32_t src[N], rows[N];  // of run i
+  int32_t first[N];         // its first destination, and (top 8 bits) how many it has
+  int32_t dst[N];
 };
 
-// Tasks of 4 KB: (copy, layer x head, K or V, piece of the page's rows). Every lane has its eight
-// 16-byte loads in flight before the first store. Bound by HBM: each byte is read and written once.
-__global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ KvCopyList list, int n, uint4* __restrict__ k,
+// Tasks of 4 KB: (run, layer x head, K or V, piece of the page's rows). Every lane has its eight 16-byte loads
+// in flight before the first store. Bound by HBM: a byte is read once for a run and written once a copy.
+template <int N>
+__global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ KvCopyList<N> list, int n, uint4* __restrict__ k,
                                                       uint4* __restrict__ v, int blocks, int num_pages, int page16, int row16, int pieces) {
   const int lane = threadIdx.x & 31;
   const long long warps = (long long)gridDim.x * 8;
@@ -899,52 +905,76 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Kv
     const int kv = (int)(x & 1);
     x >>= 1;
     const int b = (int)(x % blocks), i = (int)(x / blocks);
-    const PageCopy c = list.c[i];
-    const int end = c.rows * row16;
+    const int end = list.rows[i] * row16;
     const int at = piece * 256 + lane;
     if (piece * 256 >= end) continue;
     uint4* base = (kv ? v : k) + (size_t)b * num_pages * page16;
-    const uint4* src = base + (size_t)c.src * page16;
-    uint4* dst = base + (size_t)c.dst * page16;
+    const uint4* src = base + (size_t)list.src[i] * page16;
     uint4 r[8];
 #pragma unroll
     for (int e = 0; e < 8; e++)
       if (at + e * 32 < end) r[e] = __ldcs(src + at + e * 32);
+    const int first = list.first[i] & 0xFFFFFF, last = first + (list.first[i] >> 24);
+#pragma unroll 1
+    for (int j = first; j < last; j++) {
+      uint4* dst = base + (size_t)list.dst[j] * page16;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (at + e * 32 < end) dst[at + e * 32] = r[e];
+      for (int e = 0; e < 8; e++)
+        if (at + e * 32 < end) __stcs(dst + at + e * 32, r[e]);
+    }
   }
+}
+
+template <int N>
+static void launch_copies_t(void* k, void* v, int blocks, int hd, int page, int num_pages, const PageCopy* c, int m, int num_sms, cudaStream_t s) {
+  const int row16 = hd / 8;
+  KvCopyList<N> list;
+  int runs = 0, rows = 0;
+  for (int e = 0; e < m; e++) {
+    list.dst[e] = c[e].dst;
+    if (runs && c[e].src == list.src[runs - 1] && c[e].rows == list.rows[runs - 1] && (list.first[runs - 1] >> 24) < KV_RUN) {
+      list.first[runs - 1] += 1 << 24;
+      continue;
+    }
+    list.src[runs] = c[e].src;
+    list.rows[runs] = c[e].rows;
+    list.first[runs++] = e | 1 << 24;
+    rows = std::max(rows, (int)c[e].rows);
+  }
+  if (rows == 0) return;
+  const int pieces = (rows * row16 + 255) / 256;
+  const long long tasks = (long long)runs * blocks * 2 * pieces;
+  const int grid = (int)std::min<long long>((tasks + 7) / 8, (long long)num_sms * 8);
+  kv_copy_kernel<N><<<grid, 256, 0, s>>>(list, runs, reinterpret_cast<uint4*>(k), reinterpret_cast<uint4*>(v), blocks, num_pages, page * row16,
+                                         row16, pieces);
+  LS_CUDA(cudaGetLastError());
 }
 
 void launch_page_copies(void* k, void* v, int layers, int kv_heads, int hd, int page, int num_pages, const PageCopy* c, size_t n,
                         int num_sms, cudaStream_t s) {
-  const int row16 = hd / 8;
-  for (size_t i = 0; i < n; i += KV_COPIES) {
-    KvCopyList list;
-    const int m = (int)std::min<size_t>(KV_COPIES, n - i);
-    int rows = 0;
-    for (int e = 0; e < m; e++) {
-      list.c[e] = c[i + e];
-      rows = std::max(rows, (int)c[i + e].rows);
-    }
-    if (rows == 0) continue;
-    const int pieces = (rows * row16 + 255) / 256, blocks = layers * kv_heads;
-    const long long tasks = (long long)m * blocks * 2 * pieces;
-    const int grid = (int)std::min<long long>((tasks + 7) / 8, (long long)num_sms * 8);
-    kv_copy_kernel<<<grid, 256, 0, s>>>(list, m, reinterpret_cast<uint4*>(k), reinterpret_cast<uint4*>(v), blocks, num_pages, page * row16,
-                                        row16, pieces);
-    LS_CUDA(cudaGetLastError());
+  const int blocks = layers * kv_heads;
+  if (n <= KV_FEW_COPIES) return launch_copies_t<KV_FEW_COPIES>(k, v, blocks, hd, page, num_pages, c, (int)n, num_sms, s);
+  for (size_t i = 0; i < n; i += KV_COPIES)
+    launch_copies_t<KV_COPIES>(k, v, blocks, hd, page, num_pages, c + i, (int)std::min<size_t>(KV_COPIES, n - i), num_sms, s);
+}
+
+// The staged parts of a step (host memory that the device reads): block i < n, a run of page-table entries; the
+// others, the plan.
+__global__ void __launch_bounds__(256) kv_stage_kernel(int32_t* __restrict__ table, const KvRange* __restrict__ ranges, int n,
+                                                       uint4* __restrict__ plan, const uint4* __restrict__ staged, int plan16) {
+  if (blockIdx.x < n) {
+    const KvRange r = ranges[blockIdx.x];
+    const int32_t* vals = reinterpret_cast<const int32_t*>(ranges + n) + r.from;
+    for (int i = threadIdx.x; i < r.n; i += 256) table[r.at + i] = vals[i];
+  } else {
+    for (int i = (blockIdx.x - n) * 256 + threadIdx.x; i < plan16; i += (gridDim.x - n) * 256) plan[i] = staged[i];
   }
 }
 
-__global__ void __launch_bounds__(128) kv_table_kernel(int32_t* __restrict__ table, const KvRange* __restrict__ ranges, int n) {
-  const KvRange r = ranges[blockIdx.x];
-  const int32_t* vals = reinterpret_cast<const int32_t*>(ranges + n) + r.from;
-  for (int i = threadIdx.x; i < r.n; i += 128) table[r.at + i] = vals[i];
-}
-
-void launch_table_update(int32_t* table, const KvRange* ranges, int nranges, cudaStream_t s) {
-  kv_table_kernel<<<nranges, 128, 0, s>>>(table, ranges, nranges);
+void launch_stage(int32_t* table, const KvRange* ranges, int nranges, void* plan, const void* staged, size_t plan_bytes, cudaStream_t s) {
+  const int plan16 = (int)(plan_bytes / 16);
+  kv_stage_kernel<<<nranges + std::min(64, (plan16 + 255) / 256), 256, 0, s>>>(table, ranges, nranges, static_cast<uint4*>(plan),
+                                                                              static_cast<const uint4*>(staged), plan16);
   LS_CUDA(cudaGetLastError());
 }
 

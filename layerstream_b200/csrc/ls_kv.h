@@ -29,7 +29,8 @@ void launch_page_copies(void* k, void* v, int layers, int kv_heads, int hd, int 
 struct KvRange {
   int32_t at, from, n, pad;
 };
-void launch_table_update(int32_t* table, const KvRange* ranges, int nranges, cudaStream_t s);
+// The entries and the plan out of host memory that the device can read (plan_bytes a multiple of 16).
+void launch_stage(int32_t* table, const KvRange* ranges, int nranges, void* plan, const void* staged, size_t plan_bytes, cudaStream_t s);
 
 // ---- attention over shared pages: the plan ------------------------------------------------------
 //

@@ -90,7 +90,7 @@ struct LsKv {
   std::vector<std::pair<int, int>> dirty;  // [first, last) logical pages per sequence
   // staging: pinned buffers taken in turn, an event behind each upload
   struct Stage {
-    uint8_t* p = nullptr;
+    uint8_t *p = nullptr, *d = nullptr;  // host and device address
     size_t cap = 0;
     cudaEvent_t done = nullptr;
   } stage[2];
@@ -362,7 +362,7 @@ struct LsKv {
         entries += d.second - d.first;
       }
     // staged as: plan | table ranges (KvRange each) | their entries
-    const size_t plan = (planner.bytes.size() + 15) / 16 * 16, need = plan + nr * sizeof(KvRange) + entries * 4;
+    const size_t plan = planner.bytes.size(), need = plan + nr * sizeof(KvRange) + entries * 4;
     Stage& sg = stage[turn ^= 1];
     LS_CUDA(cudaEventSynchronize(sg.done));  // its last upload has been read
     if (sg.cap < need) {
@@ -371,6 +371,7 @@ struct LsKv {
       sg.cap = 0;
       const size_t cap = std::max<size_t>(2 * need, 1 << 16);
       LS_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&sg.p), cap, cudaHostAllocMapped));
+      LS_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(&sg.d), sg.p, 0));
       sg.cap = cap;
     }
     std::memcpy(sg.p, planner.bytes.data(), planner.bytes.size());
@@ -386,12 +387,7 @@ struct LsKv {
       at += n;
       d = {0, 0};
     }
-    LS_CUDA(cudaMemcpyAsync(work.plan, sg.p, planner.bytes.size(), cudaMemcpyHostToDevice, st));
-    if (nr) {
-      void* dp = nullptr;
-      LS_CUDA(cudaHostGetDevicePointer(&dp, sg.p, 0));
-      launch_table_update(d_table, reinterpret_cast<const KvRange*>(static_cast<uint8_t*>(dp) + plan), (int)nr, st);
-    }
+    launch_stage(d_table, reinterpret_cast<const KvRange*>(sg.d + plan), (int)nr, work.plan, sg.d, plan, st);
     LS_CUDA(cudaEventRecord(sg.done, st));
   }
 
