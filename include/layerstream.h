@@ -221,6 +221,15 @@ int ls_batch_open_tp(LsModel *m, uint64_t batch, uint64_t max_ctx, uint64_t max_
 int ls_batch_free(LsBatch *b);
 int ls_batch_pos(const LsBatch *b, uint64_t seq, uint64_t *pos);
 int ls_batch_truncate(LsBatch *b, uint64_t seq, uint64_t pos);
+/* No counterpart in the reference. Every dst[i] holds the first n positions of sequence src (at most its
+ * position) in the same K/V pages, and nothing else (best-of-n sampling, many questions about one
+ * prompt: prefilled once). A page is copied when one of several holders is about to write into it, and a
+ * verify pass reads a prefix that several of its sequences share once for all of them (f16 cache, head
+ * sizes 64 and 128; other shapes read it per sequence). On a tensor-parallel batch every rank makes
+ * the call. */
+int ls_batch_fork(LsBatch *b, uint64_t src, const uint64_t *dst, uint64_t ndst, uint64_t n);
+/* Pages of the batch's pool that some sequence holds, and those that more than one holds. */
+int ls_batch_pages(const LsBatch *b, uint64_t *used, uint64_t *shared);
 /* src/model.rs:111-119 for sequence `seq`: pushes n tokens, returns the greedy token after them. */
 int ls_batch_prefill(LsBatch *b, uint64_t seq, const uint32_t *ids, uint64_t n, uint32_t *argmax);
 /* ls_verify for sequences 0..nseq-1 in one pass: blocks [nseq][M]; per sequence the accepted

@@ -112,6 +112,8 @@ _SIGS = {
                                    C.POINTER(C.c_void_p)]),
     "ls_batch_pos": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(C.c_uint64)]),
     "ls_batch_truncate": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64]),
+    "ls_batch_fork": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64]),
+    "ls_batch_pages": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "ls_batch_prefill": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.POINTER(C.c_uint32)]),
     "ls_batch_verify": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p]),
     "ls_batch_spec": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64,
@@ -336,6 +338,17 @@ class Batch:
 
     def truncate(self, seq: int, pos: int):
         _check(lib().ls_batch_truncate(self._h, seq, pos))
+
+    def fork(self, src: int, dst, n: int | None = None):
+        """dst (one sequence or several) hold the first n positions of src (None: all), in the same K/V pages;
+        verify passes then read the shared prefix once for all of its sequences."""
+        d = array("Q", [dst] if isinstance(dst, int) else dst)
+        _check(lib().ls_batch_fork(self._h, src, d.buffer_info()[0], len(d), self.pos(src) if n is None else n))
+
+    def pages(self) -> dict:
+        u, s = C.c_uint64(), C.c_uint64()
+        _check(lib().ls_batch_pages(self._h, C.byref(u), C.byref(s)))
+        return {"used": u.value, "shared": s.value}
 
     def prefill(self, seq: int, ids) -> int:
         a = _u32(ids)

@@ -20,6 +20,7 @@
 
 #include "layerstream.h"
 #include "ls_internal.h"
+#include "ls_kv.h"
 
 using namespace ls;
 
@@ -53,11 +54,16 @@ int kv_page_shift() {
 // sequence's table of pool pages (a pinned host mirror and the device copy the kernels read), and
 // the number of logical pages each sequence holds. A sequence takes pages as it grows (ensure) and
 // returns those past its length when it is rolled back (shrink): a rollback is a length, and the
-// freed pages serve the next growth of any sequence. Table uploads are stream-ordered before the
+// freed pages serve the next growth of any sequence. Sequences forked from one another hold the same
+// pages (ref counts their holders); a page is copied before one of several holders writes into it
+// (own_rows), and goes back with its last holder. Table uploads are stream-ordered before the
 // pass that reads them; the host changes the mirror only between passes it has synchronized.
 struct PagePool {
   int shift = 6, nseq = 0, max_pages = 0, num_pages = 0;
   std::vector<int32_t> free_list;
+  std::vector<int32_t> ref;    // sequences holding each page
+  int nshared = 0;             // pages held by more than one
+  uint64_t version = 0;        // changes with every change of a table but growth at its end
   std::vector<int> held;       // logical pages per sequence
   int32_t* h_table = nullptr;  // [nseq][max_pages], pinned
   int32_t* d_table = nullptr;
@@ -71,8 +77,28 @@ struct PagePool {
     h_table = host_table;
     d_table = dev_table;
     held.assign(nseq, 0);
+    ref.assign(num_pages, 0);
     free_list.clear();
     for (int p = num_pages - 1; p >= 0; p--) free_list.push_back(p);  // page 0 handed out first
+  }
+  int32_t* row(int s) const { return h_table + (size_t)s * max_pages; }
+  int32_t take() {
+    const int32_t p = free_list.back();
+    free_list.pop_back();
+    ref[p] = 1;
+    return p;
+  }
+  void hold(int32_t p) {
+    if (ref[p]++ == 1) nshared++;
+  }
+  void drop(int32_t p) {
+    if (--ref[p] == 0) free_list.push_back(p);
+    else if (ref[p] == 1) nshared--;
+  }
+  void upload(int s, int first, int last, cudaStream_t st) {
+    const size_t off = (size_t)s * max_pages + first, bytes = (size_t)(last - first) * 4;
+    LS_CUDA(cudaMemcpyAsync(d_table + off, h_table + off, bytes, cudaMemcpyHostToDevice, st));
+    if (h2d) *h2d += bytes;
   }
   // Sequence s holds the pages of positions [0, n).
   void ensure(int s, size_t n, cudaStream_t st) {
@@ -80,19 +106,39 @@ struct PagePool {
     if (need <= held[s]) return;
     if (need > max_pages || (int)free_list.size() < need - held[s]) LS_THROW(LS_ERR_ARG, "the K/V page pool is exhausted");
     const int first = held[s];
-    for (int i = first; i < need; i++) {
-      h_table[(size_t)s * max_pages + i] = free_list.back();
-      free_list.pop_back();
-    }
+    for (int i = first; i < need; i++) row(s)[i] = take();
     held[s] = need;
-    const size_t off = (size_t)s * max_pages + first, bytes = (size_t)(need - first) * 4;
-    LS_CUDA(cudaMemcpyAsync(d_table + off, h_table + off, bytes, cudaMemcpyHostToDevice, st));
-    if (h2d) *h2d += bytes;
+    upload(s, first, need, st);
   }
   // Sequence s keeps only the pages of positions [0, n).
   void shrink(int s, size_t n) {
     const int keep = (int)((n + page() - 1) >> shift);
-    while (held[s] > keep) free_list.push_back(h_table[(size_t)s * max_pages + --held[s]]);
+    while (held[s] > keep) drop(row(s)[--held[s]]);
+  }
+  // Sequence d holds the first n positions of sequence s, in the same pages, and nothing else.
+  void fork(int s, int d, size_t n, cudaStream_t st) {
+    const int need = (int)((n + page() - 1) >> shift);
+    for (int i = 0; i < need; i++) hold(row(s)[i]);
+    shrink(d, 0);
+    std::copy(row(s), row(s) + need, row(d));
+    held[d] = need;
+    version++;
+    if (need) upload(d, 0, need, st);
+  }
+  // Before sequence s (n positions) writes positions [n, end): of its pages there, those that others
+  // hold too are replaced by new ones, their rows in use to be copied. (The pool never runs out: it has
+  // a page for every table entry, and two entries that share one leave one over.)
+  void own_rows(int s, size_t n, size_t end, std::vector<PageCopy>& copies, cudaStream_t st) {
+    const int last = std::min(held[s], (int)((end + page() - 1) >> shift));
+    for (int i = (int)(n >> shift); nshared && i < last; i++) {
+      const int32_t old = row(s)[i];
+      if (ref[old] == 1) continue;
+      row(s)[i] = take();
+      drop(old);
+      if (n > (size_t)i << shift) copies.push_back({old, row(s)[i], (int32_t)(n - ((size_t)i << shift))});
+      version++;
+      upload(s, i, i + 1, st);
+    }
   }
   int used() const { return num_pages - (int)free_list.size(); }
 };
@@ -1547,7 +1593,13 @@ struct LsBatch {
   float* bg_partial = nullptr;
   unsigned* bg_tickets = nullptr;
   bool graphs_on = true;                       // LS_BATCH_GRAPHS=0 launches every pass eagerly
-  std::map<int, cudaGraphExec_t> bgraphs;      // decode passes by block length
+  std::map<int, cudaGraphExec_t> bgraphs;      // decode passes by block length (over shared pages: + 1 << 16)
+  // attention over pages that several sequences share (made by the first fork's pass)
+  KvWork kvw;
+  KvPlanner planner;
+  std::vector<CUtensorMap> kv_maps;            // [layers] K, V
+  uint8_t* h_plan = nullptr;
+  std::vector<PageCopy> copies;
   uint32_t *h_tok = nullptr, *h_m = nullptr, *h_next = nullptr;
   int *h_pos0 = nullptr, *h_err = nullptr;
   int inject_err = 0;      // test hook: the next pass reports this error code (a host-made fault)
@@ -1813,6 +1865,7 @@ struct LsBatch {
     // a failed tensor-parallel pass may leave collectives in flight on a peer: abort, do not wait
     if (comm) (tp_failed ? nccl_api().comm_abort : nccl_api().comm_destroy)(comm);
     for (cudaEvent_t e : prof_ev) cudaEventDestroy(e);
+    kvw.close();
     for (void* p : ipc_maps) cudaIpcCloseMemHandle(p);
     for (void* p : dev_allocs) cudaFree(p);
     for (void* p : host_allocs) cudaFreeHost(p);
@@ -2049,8 +2102,71 @@ struct LsBatch {
 
   // A sequence's length; the pages past it go back to the pool.
   void set_pos(size_t sq, uint64_t p) {
+    if (p < pos[sq]) pool.version++;
     pos[sq] = p;
     pool.shrink((int)sq, p);
+  }
+
+  // Every dst holds the first n positions of src, in the same pages: best-of-n sampling, or many questions
+  // about one document, prefilled once.
+  void fork(uint64_t src, const uint64_t* dst, uint64_t ndst, uint64_t n) {
+    if (src >= B) LS_THROW(LS_ERR_ARG, "sequence index out of range");
+    if (n > pos[src]) LS_THROW(LS_ERR_ARG, "sequence " + std::to_string(src) + " holds " + std::to_string(pos[src]) + " positions");
+    std::vector<char> seen(B, 0);
+    for (uint64_t i = 0; i < ndst; i++) {
+      if (dst[i] >= B) LS_THROW(LS_ERR_ARG, "sequence index out of range");
+      if (dst[i] == src) LS_THROW(LS_ERR_ARG, "a sequence cannot be forked onto itself");
+      if (seen[dst[i]]++) LS_THROW(LS_ERR_ARG, "sequence " + std::to_string(dst[i]) + " is named twice");
+    }
+    LS_CUDA(cudaSetDevice(m->device));
+    for (uint64_t i = 0; i < ndst; i++) {
+      pool.fork((int)src, (int)dst[i], n, stream);
+      pos[dst[i]] = n;
+    }
+    LS_CUDA(cudaStreamSynchronize(stream));  // the tables' mirror may change again
+  }
+
+  // Whether the pass of sequences s0 .. s0 + ns - 1, M rows each, reads a prefix that several of them hold in the
+  // same pages; its plan is then on the device. LS_SHARED=0: every sequence reads its own context.
+  bool plan_shared(size_t s0, size_t ns, int M) {
+    const Config& c = m->cfg;
+    const int hd = (int)c.head_dim;
+    if (!pool.nshared || ns < 2 || !use_bg || (hd != 64 && hd != 128) || ns * M > B * max_block) return false;
+    const char* e = getenv("LS_SHARED");
+    if (e && std::string(e) == "0") return false;
+    if (!kvw.mem) {
+      KvGeom g;
+      g.heads = dm.heads;
+      g.kv_heads = dm.kv_heads;
+      g.hd = hd;
+      g.shift = pool.shift;
+      g.num_pages = pool.num_pages;
+      g.max_pages = pool.max_pages;
+      g.nseq = (int)B;
+      g.max_rows = (int)(B * max_block);
+      g.nctas = m->num_sms;
+      planner.g = g;
+      h_plan = halloc<uint8_t>(g.plan_cap());
+      kv_maps.resize(2 * c.layers);
+      for (size_t l = 0; l < c.layers; l++)
+        for (int i = 0; i < 2; i++)
+          kv_encode_map(&kv_maps[2 * l + i], (i ? vc : kc) + l * kv_layer, (uint64_t)dm.kv_heads * pool.num_pages << pool.shift, hd,
+                        kv_box_rows(pool.page()), false);
+      kvw.open(g, false, d_err);
+    }
+    std::vector<KvSeqIn> in(ns);
+    for (size_t i = 0; i < ns; i++) {
+      in[i].n = (int)pos[s0 + i];
+      in[i].cnt = M;
+      in[i].table = pool.row((int)(s0 + i));
+      in[i].tab = (int)((s0 + i) * pool.max_pages);
+    }
+    planner.build(in, M, (pool.version << 24) + (s0 << 12) + ns);
+    if (planner.shared_positions() == 0) return false;
+    std::memcpy(h_plan, planner.bytes.data(), planner.bytes.size());
+    LS_CUDA(cudaMemcpyAsync(kvw.plan, h_plan, planner.bytes.size(), cudaMemcpyHostToDevice, stream));
+    h2d_bytes += planner.bytes.size();
+    return true;
   }
 
   void pass(size_t s0, size_t ns, int M, const uint32_t* tokens, int head_mode) {
@@ -2070,7 +2186,15 @@ struct LsBatch {
     }
     for (size_t i = 0; i < T; i++)
       if (tokens[i] >= c.vocab) LS_THROW(LS_ERR_ARG, "token id " + std::to_string(tokens[i]) + " is outside the vocabulary");
-    for (size_t i = 0; i < ns; i++) pool.ensure((int)(s0 + i), pos[s0 + i] + M, stream);  // pages for the new rows
+    copies.clear();
+    for (size_t i = 0; i < ns; i++) {  // pages for the new rows, none of them anyone else's
+      pool.own_rows((int)(s0 + i), pos[s0 + i], pos[s0 + i] + M, copies, stream);
+      pool.ensure((int)(s0 + i), pos[s0 + i] + M, stream);
+    }
+    if (!copies.empty())
+      launch_page_copies(kc, vc, (int)c.layers, dm.kv_heads, (int)c.head_dim, pool.page(), pool.num_pages, copies.data(), copies.size(),
+                         m->num_sms, stream);
+    const bool over_shared = plan_shared(s0, ns, M);
     std::memcpy(h_tok, tokens, T * 4);
     h2d_bytes += T * 4 + ns * 4;
     const bool streamed = m->mode != LS_MODE_RESIDENT;
@@ -2131,13 +2255,30 @@ struct LsBatch {
       a.pdl = use_bg;  // positions come from the pass's host upload, before every kernel
       a.err = d_err;
       a.max_total = (int)span;
-      if (use_bg && attention_tc_supported(a)) {  // straight into the O GEMM's operand
+      if (use_bg && (over_shared || attention_tc_supported(a))) {  // straight into the O GEMM's operand
         int gn = 16, gg = 1;
         bgemm_groups((int)T, &gn, &gg);
         a.out_h = bt_a;
         a.out_h_n = gn;
       }
-      launch_attention(a, stream);
+      if (over_shared) {
+        KvAttn k;
+        k.qkv = qkv;
+        k.qkv_stride = QS;
+        k.qkv_f32 = true;
+        k.rope = rope;
+        k.k = kc + l * kv_layer;
+        k.v = vc + l * kv_layer;
+        k.tables = pool.d_table;
+        k.kmap = &kv_maps[2 * l];
+        k.vmap = &kv_maps[2 * l + 1];
+        k.out_bt = a.out_h;
+        k.out_bt_n = a.out_h_n;
+        k.rows = (int)T;
+        launch_kv_attention(kvw, k, stream);
+      } else {
+        launch_attention(a, stream);
+      }
       if (use_bg && !a.out_h) launch_bt_prep(attn, dm.q_dim, (int)T, dm.q_dim, nullptr, nullptr, 0.f, bt_a, stream);
       prof_end(pi);
       pi = prof_begin(2, qbytes(W.o) + act * (dm.q_dim + 2 * h));
@@ -2252,7 +2393,8 @@ struct LsBatch {
     LS_CUDA(cudaMemcpyAsync(h_err, d_err, 4, cudaMemcpyDeviceToHost, stream));
     };
     if (graphed) {
-      auto it = bgraphs.find(M);
+      const int key = M + (over_shared ? 1 << 16 : 0);
+      auto it = bgraphs.find(key);
       if (it == bgraphs.end()) {
         cudaGraph_t graph;
         LS_CUDA(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
@@ -2266,7 +2408,7 @@ struct LsBatch {
         cudaGraphExec_t exec;
         LS_CUDA(cudaGraphInstantiate(&exec, graph, 0));
         cudaGraphDestroy(graph);
-        it = bgraphs.emplace(M, exec).first;
+        it = bgraphs.emplace(key, exec).first;
       }
       LS_CUDA(cudaGraphLaunch(it->second, stream));
     } else {
@@ -3018,6 +3160,22 @@ int ls_batch_truncate(LsBatch* b, uint64_t seq, uint64_t pos) {
     if (seq >= b->B) LS_THROW(LS_ERR_ARG, "sequence index out of range");
     if (pos > b->pos[seq]) LS_THROW(LS_ERR_ARG, "cannot truncate to a position beyond the cache");
     b->set_pos(seq, pos);
+  });
+}
+
+int ls_batch_fork(LsBatch* b, uint64_t src, const uint64_t* dst, uint64_t ndst, uint64_t n) {
+  return guard([&] {
+    NEED(b);
+    if (ndst) NEED(dst);
+    b->fork(src, dst, ndst, n);
+  });
+}
+
+int ls_batch_pages(const LsBatch* b, uint64_t* used, uint64_t* shared) {
+  return guard([&] {
+    NEED(b);
+    if (used) *used = (uint64_t)b->pool.used();
+    if (shared) *shared = (uint64_t)b->pool.nshared;
   });
 }
 
