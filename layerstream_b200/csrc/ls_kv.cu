@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   constexpr uint32_t COL_P = OVER ? 64 : 384, STEP_P = OVER ? 128 : 64, COL_O = 256;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS];
-  __shared__ uint64_t q_full[2][2], s_full[2], s_read[2], p_half[2], p_full[2], pv_done[2], o_free[2], turn;
+  __shared__ uint64_t q_full[2][2], s_full[2], s_read[2], p_full[2], pv_done[2], o_free[2], turn;
   __shared__ __align__(16) KvSeg s_segs[2][KV_SEGS_NEAR];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -358,7 +358,6 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       tc::mbar_init(&q_full[t][1], 1);
       tc::mbar_init(&s_full[t], 1);
       tc::mbar_init(&s_read[t], 4);
-      tc::mbar_init(&p_half[t], 4);
       tc::mbar_init(&p_full[t], 4);
       tc::mbar_init(&pv_done[t], 1);
       tc::mbar_init(&o_free[t], 4);
@@ -472,83 +471,72 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kv_wait(bar, parity, &s_abort)); };
       auto cols = [&](const KvSeg& s, int j) { return min(KV_CHUNK, (s.p1 - s.p0 - j * KV_CHUNK + 31) & ~31); };
       int si = 0, sj = 0, sc = 0;
-      // Chunk (i, j): round 0, its values of positions 64 .. 127 (P's upper half comes first); round 1, those of
-      // positions 0 .. 63; the next S, at hd 64 in round 1 ahead of them if its operands are there (a P V must
-      // not wait for the next chunk's copies, which may wait for the stage that it frees), else behind them in
-      // round 2. At hd 128, where P lies over S, it comes once the P V is done. Chunk -1 is round 2 alone.
+      // Chunk (i, j): round 0, at hd 64, the next S as soon as this one is in registers, if its operands are there
+      // (this chunk's P V must not wait for the next chunk's copies, which may wait for the stage that it
+      // frees); round 1, the P V, then the next S if it is still to come (at hd 128, where P lies over
+      // S, once the P V is done). Chunk -1 is the first S alone.
       int i = 0, j = 0;
       bool ok = true;
 #pragma unroll 1
       for (int chunk = -1; ok && (chunk < 0 || i < nseg); chunk++) {
         bool done = si >= nseg;  // the next S has been issued, or there is none
-        int st = 0;
-        uint32_t ph = 0;
-        if (chunk >= 0) {
-          ring(chunk, t, st, ph);
-          ok = wait(&v_full[st], ph & 1);
-          if (j == 0 && i > 0) ok = ok && wait(&o_free[t], (i - 1) & 1);
-        }
 #pragma unroll 1
-        for (int round = chunk < 0 ? 2 : 0; ok && round < 3; round++) {
-          if (round > 0 && !done) {
-            const KvSeg& s = seg_of(t, si);
-            int st_k;
-            uint32_t ph_k;
-            ring(sc, t, st_k, ph_k);
-            uint64_t* qb = &q_full[t][si & 1];
-            bool go = true;
-            if (round == 1) {
-              ok = wait(&s_read[t], chunk & 1);
-              if (sj == 0) load_ahead(si);
-              const bool q = !OVER && (sj > 0 || tc::mbar_poll(qb, (si >> 1) & 1));
-              go = __all_sync(0xffffffffu, q && tc::mbar_poll(&k_full[st_k], ph_k & 1));
-            } else {
-              if (sj == 0) load_ahead(si);
-              ok = (sj > 0 || wait(qb, (si >> 1) & 1)) && wait(&k_full[st_k], ph_k & 1);
-              if (OVER && chunk >= 0) ok = ok && wait(&pv_done[t], chunk & 1);
-            }
-            if (!ok) break;
-            if (go) {
-              tc::fence_after();
-              const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + st_k * SM::kChunk, 16);
-              const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(cols(s, sj) >> 3) << 17;
-#pragma unroll 1
-              for (int k = 0; k < HD / 16; k++)
-                kv_mma_ss(lead, t_s, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4), b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
-              kv_commit(lead, &s_full[t]);
-              kv_commit(lead, &k_empty[st_k]);
-              if (sc >= pr.pair_ch && lead) tc::mbar_arrive(&k_empty[st_k]);
-              __syncwarp();
-              done = true;
-              sc++;
-              if (++sj == s.nch) {
-                sj = 0;
-                si++;
-              }
-            }
-          }
-          if (round < 2) {
+        for (int round = chunk < 0; ok && round < 2; round++) {
+          if (round && chunk >= 0) {
             const KvSeg& s = seg_of(t, i);
+            int st;
+            uint32_t ph;
+            ring(chunk, t, st, ph);
             const int ncol = cols(s, j);
-            ok = wait(round ? &p_full[t] : &p_half[t], chunk & 1);
+            ok = wait(&v_full[st], ph & 1);
+            if (j == 0 && i > 0) ok = ok && wait(&o_free[t], (i - 1) & 1);
+            ok = ok && wait(&p_full[t], chunk & 1);
             if (!ok) break;
             tc::fence_after();
             const uint32_t b0 = kv_desc(smem + SM::kV + st * SM::kChunk, BLK);
-            const int k1 = round ? min(ncol, 64) >> 4 : ncol >> 4;
-            const bool first = j == 0 && (round == 0 || ncol <= 64);
 #pragma unroll 1
-            for (int k = round ? 0 : 4; k < k1; k++)
-              kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), !(first && (k & 3) == 0));
-            if (round == 1) {
-              kv_commit(lead, &pv_done[t]);
-              kv_commit(lead, &v_empty[st]);
-              if (chunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[st]);
-              __syncwarp();
-              if (++j == s.nch) {
-                j = 0;
-                i++;
-              }
+            for (int k = 0; k * 16 < ncol; k++)
+              kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), j > 0 || k > 0);
+            kv_commit(lead, &pv_done[t]);
+            kv_commit(lead, &v_empty[st]);
+            if (chunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[st]);
+            __syncwarp();
+            if (++j == s.nch) {
+              j = 0;
+              i++;
             }
+          }
+          if (done || (OVER && round == 0)) continue;
+          const KvSeg& s = seg_of(t, si);
+          int st;
+          uint32_t ph;
+          ring(sc, t, st, ph);
+          if (round == 0) ok = wait(&s_read[t], chunk & 1);
+          if (sj == 0) load_ahead(si);
+          uint64_t* qb = &q_full[t][si & 1];
+          if (round == 0) {
+            const bool q = sj > 0 || tc::mbar_poll(qb, (si >> 1) & 1);
+            if (!__all_sync(0xffffffffu, ok && q && tc::mbar_poll(&k_full[st], ph & 1))) continue;
+          } else {
+            ok = (sj > 0 || wait(qb, (si >> 1) & 1)) && wait(&k_full[st], ph & 1);
+            if (OVER && chunk >= 0) ok = ok && wait(&pv_done[t], chunk & 1);
+            if (!ok) break;
+          }
+          tc::fence_after();
+          const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + st * SM::kChunk, 16);
+          const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(cols(s, sj) >> 3) << 17;
+#pragma unroll 1
+          for (int k = 0; k < HD / 16; k++)
+            kv_mma_ss(lead, t_s, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4), b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
+          kv_commit(lead, &s_full[t]);
+          kv_commit(lead, &k_empty[st]);
+          if (sc >= pr.pair_ch && lead) tc::mbar_arrive(&k_empty[st]);
+          __syncwarp();
+          done = true;
+          sc++;
+          if (++sj == s.nch) {
+            sj = 0;
+            si++;
           }
         }
       }
@@ -580,47 +568,51 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     bool ok = true;
 #pragma unroll 1
     for (int i = 0; ok && i < pr.nseg[t]; i++) {
-      const KvSeg& s = seg_of(t, i);
-      const int row = quad * 32 + lane - s.shift;
-      const bool row_ok = row >= 0 && row < s.nrows;
-      const bool active = quad * 32 >= s.shift && quad * 32 < s.shift + s.nrows;  // warp-uniform
-      // last position the row sees
-      int lim = s.p1 - 1;
-      if (s.causal != INT_MAX && row_ok) lim = min(lim, s.causal + (s.trow0 + row) / a.G);
+      const KvSeg& sg = seg_of(t, i);
+      const int p0 = sg.p0, p1 = sg.p1, nch = sg.nch, causal = sg.causal;
+      const int row = quad * 32 + lane - sg.shift;
+      const bool row_ok = row >= 0 && row < sg.nrows;
+      const bool active = quad * 32 >= sg.shift && quad * 32 < sg.shift + sg.nrows;  // warp-uniform
+      // last position the row sees, and the last that all of the warp's rows see
+      int lim = p1 - 1, seen = p1 - 1;
+      if (causal != INT_MAX) {
+        if (row_ok) lim = min(lim, causal + (sg.trow0 + row) / a.G);
+        seen = min(seen, causal + (sg.trow0 + max(0, quad * 32 - sg.shift)) / a.G);
+      }
       float m_ref = -CUDART_INF_F, l = 0.f;
 #pragma unroll 1
-      for (int j = 0; j < s.nch; j++, chunk++) {
-        const int pc = s.p0 + j * KV_CHUNK;
-        const int ncol = min(KV_CHUNK, (s.p1 - pc + 31) & ~31);  // columns of S and P that the MMAs use
-        const int hi = ncol > 64;                                // the upper 64 are among them
+      for (int j = 0; j < nch; j++, chunk++) {
+        const int pc = p0 + j * KV_CHUNK;
+        const int ncol = min(KV_CHUNK, (p1 - pc + 31) & ~31);  // columns of S and P that the MMAs use
         ok = wait(&s_full[t], chunk & 1);
         if (!ok) break;
-        // S, 64 columns at a time: both halves for the maximum, then the upper half's weights from registers and
-        // the lower half's from a second read. (Loops, not unrolled: the warps' roles together should stay
-        // within the instruction caches. With the whole row unrolled, 80 KB of code, the exponentials took 2000
-        // to 4000 cycles instead of 1500 whenever all SMs were busy.)
-        float x[64];
-        const int vis = lim - pc;  // columns 0 .. vis are visible
-        const bool all = __all_sync(0xffffffffu, vis >= KV_CHUNK - 1 || !row_ok);
-        auto load_s = [&](int h) {
-          kv_ld32(t_s + h * 64, x);
-          if (ncol > h * 64 + 32) kv_ld32(t_s + h * 64 + 32, x + 32);
-          kv_wait32(x);
-          kv_wait32(x + 32);
-          if (!all) {
+        // the row's scores into registers; at hd 64 the next S may take this one's place
+        float x[128];
+        if (active) {
+          if (pc + KV_CHUNK - 1 > seen) {  // -inf into the columns that the row does not see
+            const int vis = lim - pc;
+#pragma unroll 1
+            for (int c0 = 0; c0 < KV_CHUNK; c0 += 32) {
+              kv_ld32(t_s + c0, x);
+              kv_wait32(x);
 #pragma unroll
-            for (int c = 0; c < 64; c++) x[c] = h * 64 + c <= vis ? x[c] : -CUDART_INF_F;
+              for (int c = 0; c < 32; c++) x[c] = c0 + c <= vis ? x[c] : -CUDART_INF_F;
+              tc::st16(t_s + c0, reinterpret_cast<uint32_t*>(x));
+              tc::st16(t_s + c0 + 16, reinterpret_cast<uint32_t*>(x + 16));
+            }
+            tc::wait_st();
           }
-        };
+#pragma unroll
+          for (int q = 0; q < 4; q++) kv_ld32(t_s + q * 32, x + q * 32);
+#pragma unroll
+          for (int q = 0; q < 4; q++) kv_wait32(x + q * 32);
+        }
+        if (!OVER) arrive(&s_read[t]);
         float mb = 0.f;
         if (active) {
           float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll 1
-          for (int h = 0; h <= hi; h++) {
-            load_s(h);
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = kv_max3_nan(mx[(c >> 1) & 3], x[c], x[c + 1]);
-          }
+          for (int c = 0; c < 128; c += 2) mx[(c >> 1) & 3] = kv_max3_nan(mx[(c >> 1) & 3], x[c], x[c + 1]);
           const float m_new = kv_max_nan(kv_max_nan(mx[0], mx[1]), kv_max_nan(mx[2], mx[3])) * cs;  // NaN if one score is
           if (j == 0) {
             m_ref = m_new;
@@ -653,8 +645,8 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
         }
         // V rows that nobody sees (past the range) are zeroed, and infinities and NaN of rows that
         // only some of the tile see; all four warps take part
-        const bool tail = pc + ncol > s.p1;
-        const bool fresh = s.causal != INT_MAX && s.p1 > s.causal + 1 && pc + KV_CHUNK > s.causal + 1;
+        const bool tail = pc + ncol > p1;
+        const bool fresh = causal != INT_MAX && p1 > causal + 1 && pc + KV_CHUNK > causal + 1;
         if (tail || fresh) {
           int st;
           uint32_t ph;
@@ -662,8 +654,8 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           ok = wait(&v_full[st], ph & 1);
           if (!ok) break;
           uint8_t* sv = smem_gen + SM::kV + st * SM::kChunk;
-          const int r1 = min(KV_CHUNK, s.p1 - pc);
-          const int r0 = fresh ? max(0, s.causal + 1 - pc) : r1;
+          const int r1 = min(KV_CHUNK, p1 - pc);
+          const int r0 = fresh ? max(0, causal + 1 - pc) : r1;
 #pragma unroll 1
           for (int k = quad * 32 + lane; k < (ncol - r0) * CB * 8; k += 128) {
             const int r = r0 + k / (CB * 8), c = k % (CB * 8);
@@ -675,7 +667,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
               const uint4 n = make_uint4(kv_nonfinite<BF16>(v.x), kv_nonfinite<BF16>(v.y), kv_nonfinite<BF16>(v.z), kv_nonfinite<BF16>(v.w));
               if (n.x | n.y | n.z | n.w) {
                 *p = make_uint4(v.x & ~n.x, v.y & ~n.y, v.z & ~n.z, v.w & ~n.w);
-                a.flags[s.flag] = 1;
+                a.flags[sg.flag] = 1;
               }
             }
           }
@@ -683,41 +675,33 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
         }
         // Before P is stored: the last P has been read. Warps without rows wait too, or their arrivals could count
         // for the chunk before.
-        if (chunk > 0) {
+        if (!OVER && chunk > 0) {  // (at hd 128 S itself comes after the last P V)
           ok = wait(&pv_done[t], (chunk - 1) & 1);
           if (!ok) break;
         }
         const uint64_t cs2 = kv_f2(cs, cs), mb2 = kv_f2(-mb, -mb);
         uint64_t ls[4] = {0, 0, 0, 0};
-#pragma unroll 1
-        for (int h = 1; h >= 0; h--) {
-          if (active && h < hi) load_s(h);
-          if (h == 0) arrive(&s_read[t]);  // at hd 64 the next S may take this one's place
-          if (active && h <= hi) {
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-              if (h * 64 + q * 32 >= ncol) continue;
-              uint32_t pk[16];
+        for (int q = 0; q < 4; q++)
+          if (active && q * 32 < ncol) {
+            uint32_t pk[16];
 #pragma unroll
-              for (int e = 0; e < 16; e++) {
-                const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
-                float2 w;
-                if ((e & 7) == 1 || (e & 7) == 4 || (e & 7) == 6) {
-                  w = kv_ex2_fma(z);
-                } else {
-                  w = kv_un2(z);
-                  w.x = kv_ex2(w.x);
-                  w.y = kv_ex2(w.y);
-                }
-                ls[e & 3] = kv_add2(ls[e & 3], kv_f2(w.x, w.y));
-                pk[e] = kv_pack<BF16>(w.x, w.y);
+            for (int e = 0; e < 16; e++) {
+              const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
+              float2 w;
+              if ((e & 7) == 1 || (e & 7) == 4 || (e & 7) == 6) {
+                w = kv_ex2_fma(z);
+              } else {
+                w = kv_un2(z);
+                w.x = kv_ex2(w.x);
+                w.y = kv_ex2(w.y);
               }
-              tc::st16(t_p + h * 32 + q * 16, pk);
+              ls[e & 3] = kv_add2(ls[e & 3], kv_f2(w.x, w.y));
+              pk[e] = kv_pack<BF16>(w.x, w.y);
             }
-            tc::wait_st();
+            tc::st16(t_p + q * 16, pk);
           }
-          if (h) arrive(&p_half[t]);
-        }
+        if (active) tc::wait_st();
         const float2 lf = kv_un2(kv_add2(kv_add2(ls[0], ls[1]), kv_add2(ls[2], ls[3])));
         l += lf.x + lf.y;
         arrive(&p_full[t]);
@@ -727,7 +711,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       ok = wait(&pv_done[t], (chunk - 1) & 1);
       if (!ok) break;
       if (active) {
-        float* po = a.part + ((size_t)s.slot + row) * HD;
+        float* po = a.part + ((size_t)sg.slot + row) * HD;
 #pragma unroll 1
         for (int q = 0; q < HD / 32; q++) {
           float o[32];
@@ -737,7 +721,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 4; e++) kv_st8(po + q * 32 + 8 * e, o + 8 * e);
         }
-        if (row_ok) reinterpret_cast<float2*>(a.part + (size_t)h.nslots * HD)[s.slot + row] = make_float2(m_ref, l);
+        if (row_ok) reinterpret_cast<float2*>(a.part + (size_t)h.nslots * HD)[sg.slot + row] = make_float2(m_ref, l);
       }
       arrive(&o_free[t]);
     }
