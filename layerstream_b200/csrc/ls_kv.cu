@@ -85,25 +85,6 @@ __device__ __forceinline__ float kv_max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^z on the FMA units, for the share of the exponentials that the special-function units (16 a clock and SM)
-// would be late with: z = n + f, n the nearest integer (Cody and Waite's reduction; it sits in the low bits
-// of z + 1.5 * 2^23), 2^f by the quartic with the least largest relative error on [-1/2, 1/2] (Remez
-// exchange, 2.6e-6), n added to the exponent. z is clamped at -126, so the result is at least 2^-126 (ends
-// as zero or next to it in P); z up to 8 occurs. A NaN does not come through: the row's maximum carries it.
-__device__ __forceinline__ float2 kv_ex2_fma(uint64_t z) {
-  const float2 zf = kv_un2(z);
-  z = kv_f2(fmaxf(zf.x, -126.f), fmaxf(zf.y, -126.f));
-  const uint64_t r = kv_add2(z, kv_f2(12582912.f, 12582912.f));
-  const uint64_t f = kv_fma2(kv_add2(r, kv_f2(-12582912.f, -12582912.f)), kv_f2(-1.f, -1.f), z);
-  uint64_t p = kv_f2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
-  p = kv_fma2(p, f, kv_f2(0x1.ca1444p-5f, 0x1.ca1444p-5f));
-  p = kv_fma2(p, f, kv_f2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-  p = kv_fma2(p, f, kv_f2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-  p = kv_fma2(p, f, kv_f2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  const float2 pf = kv_un2(p), rf = kv_un2(r);
-  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23)),
-                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23)));
-}
 template <bool BF16>
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
   if constexpr (BF16) {
@@ -494,9 +475,9 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
             if (!ok) break;
             tc::fence_after();
             const uint32_t b0 = kv_desc(smem + SM::kV + st * SM::kChunk, BLK);
-#pragma unroll 1
-            for (int k = 0; k * 16 < ncol; k++)
-              kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), j > 0 || k > 0);
+#pragma unroll
+            for (int k = 0; k < KV_CHUNK / 16; k++)
+              if (k * 16 < ncol) kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), j > 0 || k > 0);
             kv_commit(lead, &pv_done[t]);
             kv_commit(lead, &v_empty[st]);
             if (chunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[st]);
@@ -525,7 +506,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           tc::fence_after();
           const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + st * SM::kChunk, 16);
           const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(cols(s, sj) >> 3) << 17;
-#pragma unroll 1
+#pragma unroll
           for (int k = 0; k < HD / 16; k++)
             kv_mma_ss(lead, t_s, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4), b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
           kv_commit(lead, &s_full[t]);
@@ -688,14 +669,9 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
-              float2 w;
-              if ((e & 7) == 1 || (e & 7) == 4 || (e & 7) == 6) {
-                w = kv_ex2_fma(z);
-              } else {
-                w = kv_un2(z);
-                w.x = kv_ex2(w.x);
-                w.y = kv_ex2(w.y);
-              }
+              float2 w = kv_un2(z);
+              w.x = kv_ex2(w.x);
+              w.y = kv_ex2(w.y);
               ls[e & 3] = kv_add2(ls[e & 3], kv_f2(w.x, w.y));
               pk[e] = kv_pack<BF16>(w.x, w.y);
             }
