@@ -15,8 +15,17 @@
 //   kv_merge_kernel  per query row: O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over its partials
 //
 // Warp roles of kv_attn_kernel: two softmax warpgroups (one per lane of the CTA), one MMA issuer warp
-// per lane, one TMA producer warp. O stays in tensor memory and is rescaled only when a row's maximum
-// has grown by more than 2^8 over the one its exponents are taken against.
+// per lane, one TMA producer warp. K and V come in chunks of 128 positions; the softmax takes them by halves of
+// 64, so that a lane's two S buffers fit beside O in tensor memory at hd 128 too, and the tensor cores work
+// on one half while the softmax works on the other. (One buffer of 128 positions: 107 instead of 90 us
+// for many pair tiles at hd 128; at hd 64, where the next S could follow as soon as the last one was in
+// registers, 75 us either way.) O stays in tensor memory and is rescaled only when a row's maximum has
+// grown by more than 2^8 over the one its exponents are taken against.
+//
+// Bound, per two tiles and 128 positions: the special-function units need 2048 clocks for the exponentials
+// (1536 with a quarter of them on the FMA units), the tensor cores at hd 128 about 1500, HBM 1700 for K
+// and V; the kernel takes about 3400. The rest is the latency of a row's chain through one step (scores
+// out of tensor memory, maximum, exponentials, P into tensor memory, P V, next S).
 //
 // Rounding: q (after rotation) and P enter the tensor core in the cache's 16-bit type, the type that
 // its operands K and V have; scores, maxima, sums, O and the partials stay f32; the output is rounded
@@ -35,6 +44,7 @@
 namespace ls {
 
 constexpr int KV_THREADS = 352;  // 2 softmax warpgroups, 2 issuer warps, 1 producer warp
+constexpr int KV_HALF = KV_CHUNK / 2;  // positions that a step of the softmax takes
 constexpr int KV_SEGS_NEAR = 32;    // segments of a lane that are held in shared memory
 constexpr float KV_RESCALE = 8.0f;  // log2 growth of a row's maximum that O is rescaled for
 
@@ -42,7 +52,7 @@ template <int HD>
 struct KvSmem {
   static constexpr int kTile = KV_TILE * HD * 2;    // Q tile
   static constexpr int kChunk = KV_CHUNK * HD * 2;  // K chunk, V chunk
-  static constexpr int kStages = HD == 64 ? 4 : 2;  // of K and of V, even: in the lanes' own phase lane t owns those of parity t
+  static constexpr int kStages = HD == 64 ? 4 : 2;  // of K and of V; even: in the lanes' own phase lane t owns those of parity t
   static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kChunk;
   static constexpr int kTotal = kV + kStages * kChunk + 1024;  // + alignment
 };
@@ -84,6 +94,27 @@ __device__ __forceinline__ float kv_max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// 2^z on the FMA units, for a share of the exponentials (the special-function units do 16 a clock and SM):
+// z = n + f, n the nearest integer (Cody and Waite's reduction; it sits in the low bits of z + 1.5 * 2^23),
+// 2^f by the quartic with the least largest relative error on [-1/2, 1/2] (Remez exchange, 2.6e-6), n added
+// to the exponent. z is clamped at -126, so the result is at least 2^-126 (ends as zero or next to it
+// in P); z up to 8 occurs. A NaN does not come through: the row's maximum carries it.
+// Many pair tiles at hd 128 and 64: no share 93.7 and 79.8 us, a quarter 89.7 and 77.3, 3/8 90.4 and
+// 77.4, half 94.1 and 80.9.
+__device__ __forceinline__ float2 kv_ex2_fma(uint64_t z) {
+  const float2 zf = kv_un2(z);
+  z = kv_f2(fmaxf(zf.x, -126.f), fmaxf(zf.y, -126.f));
+  const uint64_t r = kv_add2(z, kv_f2(12582912.f, 12582912.f));
+  const uint64_t f = kv_fma2(kv_add2(r, kv_f2(-12582912.f, -12582912.f)), kv_f2(-1.f, -1.f), z);
+  uint64_t p = kv_f2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+  p = kv_fma2(p, f, kv_f2(0x1.ca1444p-5f, 0x1.ca1444p-5f));
+  p = kv_fma2(p, f, kv_f2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = kv_fma2(p, f, kv_f2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = kv_fma2(p, f, kv_f2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  const float2 pf = kv_un2(p), rf = kv_un2(r);
+  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23)),
+                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23)));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
@@ -133,7 +164,7 @@ __device__ __forceinline__ void kv_wait32(float* v) {
                : "memory");
 }
 // Bounded wait on an mbarrier phase (a second or so), false and the CTA's abort flag on timeout. The loop is
-// not unrolled: it stands in the code two dozen times.
+// not unrolled: it stands in the code many times.
 __device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
 #pragma unroll 1
   for (uint32_t i = 0; i < (1u << 22); i++) {
@@ -301,13 +332,12 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   using SM = KvSmem<HD>;
   constexpr int NS = SM::kStages, CB = HD / 64;      // CB: 64-element column blocks of a row
   constexpr uint32_t QBLK = KV_TILE * 128, BLK = KV_CHUNK * 128;  // bytes of one column block of a Q tile, of a K or V chunk
-  // tensor memory: S of lane t at 128 t, O at 256 + HD t. P (two values a column): at hd 64 at 384 + 64 t; at hd 128,
-  // where nothing is left, over the upper half of S
-  constexpr bool OVER = HD == 128;
-  constexpr uint32_t COL_P = OVER ? 64 : 384, STEP_P = OVER ? 128 : 64, COL_O = 256;
+  // Tensor memory of lane t: S of its even and odd half chunks at 128 t and 128 t + 64, P (two values a column)
+  // over the first half of the S it comes from, O at 256 + HD t.
+  constexpr uint32_t COL_O = 256;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS];
-  __shared__ uint64_t q_full[2][2], s_full[2], s_read[2], p_full[2], pv_done[2], o_free[2], turn;
+  __shared__ uint64_t q_full[2][2], s_full[2][2], p_full[2][2], pv_done[2][2], o_free[2];
   __shared__ __align__(16) KvSeg s_segs[2][KV_SEGS_NEAR];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -335,15 +365,14 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       tc::mbar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; t++) {
-      tc::mbar_init(&q_full[t][0], 1);
-      tc::mbar_init(&q_full[t][1], 1);
-      tc::mbar_init(&s_full[t], 1);
-      tc::mbar_init(&s_read[t], 4);
-      tc::mbar_init(&p_full[t], 4);
-      tc::mbar_init(&pv_done[t], 1);
+      for (int e = 0; e < 2; e++) {
+        tc::mbar_init(&q_full[t][e], 1);
+        tc::mbar_init(&s_full[t][e], 1);
+        tc::mbar_init(&p_full[t][e], 4);
+        tc::mbar_init(&pv_done[t][e], 1);
+      }
       tc::mbar_init(&o_free[t], 4);
     }
-    tc::mbar_init(&turn, 4);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -425,7 +454,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     if (nseg > 0) {
       const uint32_t lead = kv_elect();
       const uint32_t sq = smem + SM::kQ + t * SM::kTile;
-      const uint32_t t_s = tmem + t * 128, t_p = tmem + COL_P + t * STEP_P, t_o = tmem + COL_O + t * HD;
+      const uint32_t t_s = tmem + t * 128, t_o = tmem + COL_O + t * HD;
       // Query tiles: segment i's may be loaded once the S products of the segment before it are done, or, when
       // both are short and in different halves of the tile, those of the one before that (the MMA reads
       // the other half's rows too, whatever they hold: no row's result depends on another row).
@@ -449,78 +478,100 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           loaded++;
         }
       };
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kv_wait(bar, parity, &s_abort)); };
-      auto cols = [&](const KvSeg& s, int j) { return min(KV_CHUNK, (s.p1 - s.p0 - j * KV_CHUNK + 31) & ~31); };
-      int si = 0, sj = 0, sc = 0;
-      // Chunk (i, j): round 0, at hd 64, the next S as soon as this one is in registers, if its operands are there
-      // (this chunk's P V must not wait for the next chunk's copies, which may wait for the stage that it
-      // frees); round 1, the P V, then the next S if it is still to come (at hd 128, where P lies over
-      // S, once the P V is done). Chunk -1 is the first S alone.
-      int i = 0, j = 0;
+      // Half chunks in order, S of number sn, P V of number pn. S may run two ahead: into the buffer of number
+      // sn - 2, once the P V that reads that one's P is done. A P V never waits for the operands of a later S:
+      // these may be behind the stage that the P V frees. The softmax warps wait for this loop: what holds for
+      // a chunk or a segment is kept in registers.
+      int sn = 0, sseg = 0, schunk = 0, sleft = seg_of(t, 0).p1 - seg_of(t, 0).p0, sst, sh = 0;  // left: positions of the segment from here on
+      int pn = 0, pseg = 0, pchunk = 0, pleft = sleft, pst, ph = 0;
+      uint32_t sphase, pphase;
+      bool snew = true, pnew = true, ready = false;  // at a segment's start; S's operands are there
+      ring(0, t, sst, sphase);
+      ring(0, t, pst, pphase);
+      load_ahead(0);
       bool ok = true;
+      uint32_t spins = 0;
 #pragma unroll 1
-      for (int chunk = -1; ok && (chunk < 0 || i < nseg); chunk++) {
-        bool done = si >= nseg;  // the next S has been issued, or there is none
-#pragma unroll 1
-        for (int round = chunk < 0; ok && round < 2; round++) {
-          if (round && chunk >= 0) {
-            const KvSeg& s = seg_of(t, i);
-            int st;
-            uint32_t ph;
-            ring(chunk, t, st, ph);
-            const int ncol = cols(s, j);
-            ok = wait(&v_full[st], ph & 1);
-            if (j == 0 && i > 0) ok = ok && wait(&o_free[t], (i - 1) & 1);
-            ok = ok && wait(&p_full[t], chunk & 1);
-            if (!ok) break;
-            tc::fence_after();
-            const uint32_t b0 = kv_desc(smem + SM::kV + st * SM::kChunk, BLK);
-#pragma unroll
-            for (int k = 0; k < KV_CHUNK / 16; k++)
-              if (k * 16 < ncol) kv_mma_ts(lead, t_o, t_p + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), j > 0 || k > 0);
-            kv_commit(lead, &pv_done[t]);
-            kv_commit(lead, &v_empty[st]);
-            if (chunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[st]);
-            __syncwarp();
-            if (++j == s.nch) {
-              j = 0;
-              i++;
+      while (pseg < nseg) {
+        if (sseg < nseg && sn < pn + 2) {
+          uint64_t* const qb = &q_full[t][sseg & 1];
+          if (!ready) {
+            if (sn == pn) {
+              ok = (!snew || kv_wait(qb, (sseg >> 1) & 1, &s_abort)) && kv_wait(&k_full[sst], sphase & 1, &s_abort);
+              if (!__all_sync(0xffffffffu, ok)) break;
+              ready = true;
+            } else {
+              ready = !snew || (loaded > sseg && tc::mbar_poll(qb, (sseg >> 1) & 1));
+              ready = __all_sync(0xffffffffu, ready && tc::mbar_poll(&k_full[sst], sphase & 1));
             }
           }
-          if (done || (OVER && round == 0)) continue;
-          const KvSeg& s = seg_of(t, si);
-          int st;
-          uint32_t ph;
-          ring(sc, t, st, ph);
-          if (round == 0) ok = wait(&s_read[t], chunk & 1);
-          if (sj == 0) load_ahead(si);
-          uint64_t* qb = &q_full[t][si & 1];
-          if (round == 0) {
-            const bool q = sj > 0 || tc::mbar_poll(qb, (si >> 1) & 1);
-            if (!__all_sync(0xffffffffu, ok && q && tc::mbar_poll(&k_full[st], ph & 1))) continue;
-          } else {
-            ok = (sj > 0 || wait(qb, (si >> 1) & 1)) && wait(&k_full[st], ph & 1);
-            if (OVER && chunk >= 0) ok = ok && wait(&pv_done[t], chunk & 1);
-            if (!ok) break;
-          }
-          tc::fence_after();
-          const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + st * SM::kChunk, 16);
-          const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(cols(s, sj) >> 3) << 17;
+          if (ready) {
+            ok = sn < 2 || kv_wait(&pv_done[t][sn & 1], ((sn - 2) >> 1) & 1, &s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc::fence_after();
+            const uint32_t a0 = kv_desc(sq, 16), b0 = kv_desc(smem + SM::kK + sst * SM::kChunk + sh * (KV_HALF * 128), 16);
+            const uint32_t id = kv_idesc<BF16>(0, false) | (uint32_t)(min(KV_HALF, (sleft + 31) & ~31) >> 3) << 17;
 #pragma unroll
-          for (int k = 0; k < HD / 16; k++)
-            kv_mma_ss(lead, t_s, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4), b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
-          kv_commit(lead, &s_full[t]);
-          kv_commit(lead, &k_empty[st]);
-          if (sc >= pr.pair_ch && lead) tc::mbar_arrive(&k_empty[st]);
-          __syncwarp();
-          done = true;
-          sc++;
-          if (++sj == s.nch) {
-            sj = 0;
-            si++;
+            for (int k = 0; k < HD / 16; k++)
+              kv_mma_ss(lead, t_s + (sn & 1) * KV_HALF, a0 + (((k >> 2) * QBLK + (k & 3) * 32u) >> 4),
+                        b0 + (((k >> 2) * BLK + (k & 3) * 32u) >> 4), id, k > 0);
+            kv_commit(lead, &s_full[t][sn & 1]);
+            sn++;
+            sleft -= KV_HALF;
+            snew = sleft <= 0;
+            if (snew || sh) {  // the chunk's last
+              kv_commit(lead, &k_empty[sst]);
+              if (schunk >= pr.pair_ch && lead) tc::mbar_arrive(&k_empty[sst]);
+              sh = 0;
+              ready = false;
+              ring(++schunk, t, sst, sphase);
+              if (snew && ++sseg < nseg) sleft = seg_of(t, sseg).p1 - seg_of(t, sseg).p0;
+            } else {
+              sh = 1;
+            }
+            spins = 0;
+            continue;
+          }
+          // the S is still to come: take the P V if that is ready
+          if (!__all_sync(0xffffffffu, tc::mbar_poll(&p_full[t][pn & 1], (pn >> 1) & 1))) {
+            ok = ++spins < (1u << 24) && ((spins & 63) || !*(volatile int*)&s_abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+              s_abort = 1;
+              ok = false;
+              break;
+            }
+            continue;
           }
         }
+        ok = ph || kv_wait(&v_full[pst], pphase & 1, &s_abort);
+        if (pnew && pseg > 0) ok = ok && kv_wait(&o_free[t], (pseg - 1) & 1, &s_abort);
+        ok = ok && kv_wait(&p_full[t][pn & 1], (pn >> 1) & 1, &s_abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc::fence_after();
+        const uint32_t b0 = kv_desc(smem + SM::kV + pst * SM::kChunk + ph * (KV_HALF * 128), BLK);
+        const uint32_t tp = t_s + (pn & 1) * KV_HALF;
+#pragma unroll
+        for (int k = 0; k < KV_HALF / 16; k++)
+          if (k < 2 || pleft > 32) kv_mma_ts(lead, t_o, tp + k * 8, b0 + k * (2048u >> 4), kv_idesc<BF16>(HD, true), !pnew || k > 0);
+        kv_commit(lead, &pv_done[t][pn & 1]);
+        pn++;
+        pleft -= KV_HALF;
+        pnew = pleft <= 0;
+        if (pnew || ph) {
+          kv_commit(lead, &v_empty[pst]);
+          if (pchunk >= pr.pair_ch && lead) tc::mbar_arrive(&v_empty[pst]);
+          ph = 0;
+          ring(++pchunk, t, pst, pphase);
+          if (pnew && ++pseg < nseg) {
+            pleft = seg_of(t, pseg).p1 - seg_of(t, pseg).p0;
+            load_ahead(pseg);
+          }
+        } else {
+          ph = 1;
+        }
+        spins = 0;
       }
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) {  // the query tiles in flight land, the MMAs in flight end
         int never = 0;
         for (int i = max(0, loaded - 2); i < loaded; i++) (void)kv_wait(&q_full[t][i & 1], (i >> 1) & 1, &never);
@@ -533,7 +584,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     // ---- softmax of lane t: one query row per thread ----
     const int t = warp >> 2, quad = warp & 3;
     const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = at + t * 128, t_p = at + COL_P + t * STEP_P, t_o = at + COL_O + t * HD;
+    const uint32_t t_o = at + COL_O + t * HD;
     const float cs = 1.4426950408889634f / sqrtf((float)HD);
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       const bool done = __all_sync(0xffffffffu, kv_wait(bar, parity, &s_abort));
@@ -545,12 +596,12 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(bar);
     };
-    int chunk = 0;
+    int chunk = 0, n = 0;  // n: the lane's half chunk
     bool ok = true;
 #pragma unroll 1
     for (int i = 0; ok && i < pr.nseg[t]; i++) {
       const KvSeg& sg = seg_of(t, i);
-      const int p0 = sg.p0, p1 = sg.p1, nch = sg.nch, causal = sg.causal;
+      const int p0 = sg.p0, p1 = sg.p1, causal = sg.causal;
       const int row = quad * 32 + lane - sg.shift;
       const bool row_ok = row >= 0 && row < sg.nrows;
       const bool active = quad * 32 >= sg.shift && quad * 32 < sg.shift + sg.nrows;  // warp-uniform
@@ -562,47 +613,37 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       }
       float m_ref = -CUDART_INF_F, l = 0.f;
 #pragma unroll 1
-      for (int j = 0; j < nch; j++, chunk++) {
-        const int pc = p0 + j * KV_CHUNK;
-        const int ncol = min(KV_CHUNK, (p1 - pc + 31) & ~31);  // columns of S and P that the MMAs use
-        ok = wait(&s_full[t], chunk & 1);
+      for (int pc = p0; pc < p1; pc += KV_HALF, n++) {
+        const int half = (pc - p0) & KV_HALF;
+        const int ncol = min(KV_HALF, (p1 - pc + 31) & ~31);  // columns of S and P that the MMAs use
+        const uint32_t t_s = at + t * 128 + (n & 1) * KV_HALF;
+        ok = wait(&s_full[t][n & 1], (n >> 1) & 1);
         if (!ok) break;
-        // the row's scores into registers; at hd 64 the next S may take this one's place
-        float x[128];
-        if (active) {
-          if (pc + KV_CHUNK - 1 > seen) {  // -inf into the columns that the row does not see
-            const int vis = lim - pc;
-#pragma unroll 1
-            for (int c0 = 0; c0 < KV_CHUNK; c0 += 32) {
-              kv_ld32(t_s + c0, x);
-              kv_wait32(x);
-#pragma unroll
-              for (int c = 0; c < 32; c++) x[c] = c0 + c <= vis ? x[c] : -CUDART_INF_F;
-              tc::st16(t_s + c0, reinterpret_cast<uint32_t*>(x));
-              tc::st16(t_s + c0 + 16, reinterpret_cast<uint32_t*>(x + 16));
-            }
-            tc::wait_st();
-          }
-#pragma unroll
-          for (int q = 0; q < 4; q++) kv_ld32(t_s + q * 32, x + q * 32);
-#pragma unroll
-          for (int q = 0; q < 4; q++) kv_wait32(x + q * 32);
-        }
-        if (!OVER) arrive(&s_read[t]);
+        float x[KV_HALF];  // the row's scores
         float mb = 0.f;
         if (active) {
+#pragma unroll
+          for (int q = 0; q < 2; q++) kv_ld32(t_s + q * 32, x + q * 32);
+#pragma unroll
+          for (int q = 0; q < 2; q++) kv_wait32(x + q * 32);
+          if (pc + KV_HALF - 1 > seen) {  // -inf into the columns that the row does not see
+            const int vis = lim - pc;
+#pragma unroll
+            for (int c = 0; c < KV_HALF; c++) x[c] = c <= vis ? x[c] : -CUDART_INF_F;
+          }
           float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-          for (int c = 0; c < 128; c += 2) mx[(c >> 1) & 3] = kv_max3_nan(mx[(c >> 1) & 3], x[c], x[c + 1]);
+          for (int c = 0; c < KV_HALF; c += 2) mx[(c >> 1) & 3] = kv_max3_nan(mx[(c >> 1) & 3], x[c], x[c + 1]);
           const float m_new = kv_max_nan(kv_max_nan(mx[0], mx[1]), kv_max_nan(mx[2], mx[3])) * cs;  // NaN if one score is
-          if (j == 0) {
+          if (pc == p0) {
             m_ref = m_new;
-          } else if (__any_sync(0xffffffffu, row_ok && !(m_new <= m_ref + KV_RESCALE))) {
-            // O and l to the new maximum, once the last P V has been added
-            ok = wait(&pv_done[t], (chunk - 1) & 1);
+          } else if (const bool grow = row_ok && !(m_new <= m_ref + KV_RESCALE); __any_sync(0xffffffffu, grow)) {
+            // O and l to the new maximum, once the last P V has been added (of the rows that it has grown in
+            // alone: what a row comes to does not depend on the others of its tile)
+            ok = wait(&pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1);
             if (!ok) break;
-            const float m2 = kv_max_nan(m_ref, m_new);
-            const float f = m2 == -CUDART_INF_F ? 1.f : kv_ex2(m_ref - m2);
+            const float m2 = grow ? kv_max_nan(m_ref, m_new) : m_ref;
+            const float f = grow ? kv_ex2(m_ref - m2) : 1.f;
             m_ref = m2;
             l *= f;
 #pragma unroll 1
@@ -618,24 +659,19 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           // the exponents' base: 0 for a row that has seen nothing yet, NaN (and so the row's weights) for a
           // maximum that is infinite or NaN
           mb = m_ref == -CUDART_INF_F ? 0.f : m_ref + (m_ref - m_ref);
-          // lane 1 starts half a step behind: one lane's MMAs and waits then run under the other's exponentials
-          if (t == 1 && chunk == 0 && pr.pair_ch > 0) {
-            ok = wait(&turn, 0);
-            if (!ok) break;
-          }
         }
         // V rows that nobody sees (past the range) are zeroed, and infinities and NaN of rows that
         // only some of the tile see; all four warps take part
         const bool tail = pc + ncol > p1;
-        const bool fresh = causal != INT_MAX && p1 > causal + 1 && pc + KV_CHUNK > causal + 1;
+        const bool fresh = causal != INT_MAX && p1 > causal + 1 && pc + KV_HALF > causal + 1;
         if (tail || fresh) {
           int st;
           uint32_t ph;
           ring(chunk, t, st, ph);
           ok = wait(&v_full[st], ph & 1);
           if (!ok) break;
-          uint8_t* sv = smem_gen + SM::kV + st * SM::kChunk;
-          const int r1 = min(KV_CHUNK, p1 - pc);
+          uint8_t* sv = smem_gen + SM::kV + st * SM::kChunk + half * 128;
+          const int r1 = min(KV_HALF, p1 - pc);
           const int r0 = fresh ? max(0, causal + 1 - pc) : r1;
 #pragma unroll 1
           for (int k = quad * 32 + lane; k < (ncol - r0) * CB * 8; k += 128) {
@@ -654,37 +690,36 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        // Before P is stored: the last P has been read. Warps without rows wait too, or their arrivals could count
-        // for the chunk before.
-        if (!OVER && chunk > 0) {  // (at hd 128 S itself comes after the last P V)
-          ok = wait(&pv_done[t], (chunk - 1) & 1);
-          if (!ok) break;
-        }
         const uint64_t cs2 = kv_f2(cs, cs), mb2 = kv_f2(-mb, -mb);
         uint64_t ls[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int q = 0; q < 2; q++)
           if (active && q * 32 < ncol) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
               const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
-              float2 w = kv_un2(z);
-              w.x = kv_ex2(w.x);
-              w.y = kv_ex2(w.y);
+              float2 w;
+              if ((e & 3) == 2) {
+                w = kv_ex2_fma(z);
+              } else {
+                w = kv_un2(z);
+                w.x = kv_ex2(w.x);
+                w.y = kv_ex2(w.y);
+              }
               ls[e & 3] = kv_add2(ls[e & 3], kv_f2(w.x, w.y));
               pk[e] = kv_pack<BF16>(w.x, w.y);
             }
-            tc::st16(t_p + q * 16, pk);
+            tc::st16(t_s + q * 16, pk);
           }
         if (active) tc::wait_st();
         const float2 lf = kv_un2(kv_add2(kv_add2(ls[0], ls[1]), kv_add2(ls[2], ls[3])));
         l += lf.x + lf.y;
-        arrive(&p_full[t]);
-        if (t == 0 && chunk == 0 && lane == 0) tc::mbar_arrive(&turn);
+        arrive(&p_full[t][n & 1]);
+        if (half || pc + KV_HALF >= p1) chunk++;
       }
       if (!ok) break;
-      ok = wait(&pv_done[t], (chunk - 1) & 1);
+      ok = wait(&pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1);
       if (!ok) break;
       if (active) {
         float* po = a.part + ((size_t)sg.slot + row) * HD;
