@@ -264,13 +264,15 @@ struct KvArgs {
 // on for q and k, 16 consecutive ones for v. Latency-bound: every row is read and written once.
 template <bool BF16, bool F32>
 __global__ void __launch_bounds__(256) kv_prep_kernel(const KvArgs a) {
+  // The rows are there, the last call's kernels have read what is overwritten here, and the step's plan is: the
+  // attention and merge kernels read it before they wait for anything, so they may start from here on.
+  pdl_wait();
   pdl_trigger();
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvSeq* sq = reinterpret_cast<const KvSeq*>(a.plan + h.off_seq);
   const int G = a.G, kvh = a.kv_heads, H = G * kvh, hd = a.hd, half = hd / 2, per = hd / 16;
   const int units = (H + 2 * kvh) * per;
   const int M = h.M;
-  pdl_wait();  // the rows; and the last call's kernels have read what is overwritten here
   const size_t total = (size_t)h.nseq * M * units;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
     const int row = (int)(i / units), u = (int)(i - (size_t)row * units);
@@ -753,123 +755,144 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
 // ---- the partials ---------------------------------------------------------------------------------
 
 // A query row's partials: their maximum, then their weighted sum, in plan order (the result does not
-// depend on timing). One warp per row, or, when the plan says that some row has many partials, the
-// block's four warps per row, each with every fourth of them. Bound by L2's latency when there are few rows
-// (sequence, units, then the maxima and four partials at once: three round trips), by its bandwidth
-// when there are many. BT: f16 in the batched GEMM's operand layout.
-template <int HD, bool BF16, bool BT>
-__global__ void __launch_bounds__(128) kv_merge_kernel(const KvArgs a) {
-  constexpr int W = HD / 32;  // f32 per lane
+// depend on timing). One warp per row and head, or, when the plan says so (few rows, some with many
+// partials), the block's four warps, each with every fourth of them (SPLIT). Bound by L2's latency when there
+// are few rows (sequence, units, then the maxima and four partials at once: three round trips, 3.5 us), by
+// L2's bandwidth when there are many (4608 rows with 10 partials of 512 bytes: 6.8 us). Eight partials in
+// flight take registers, and so warps, away: 288 rows of 16 heads 9.0 against 8.2 us, 1024 rows of
+// 14 heads 12.1 against 10.8; so does a kernel not held to 64 registers (22.1 against 23.4 us for the three
+// launches at 4608 rows). BT: f16 in the batched GEMM's operand layout.
+template <int HD, bool BF16, bool BT, bool SPLIT>
+__device__ __forceinline__ void kv_merge(const KvArgs& a, float (*s_acc)[HD], float2* s_ml) {
+  constexpr int W = HD / 32, U = 4;  // f32 per lane, partials in flight
   using V = std::conditional_t<W == 4, float4, float2>;
-  __shared__ __align__(16) float s_acc[4][HD];
-  pdl_trigger();
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvSeq* sqs = reinterpret_cast<const KvSeq*>(a.plan + h.off_seq);
   const KvUnit* units = reinterpret_cast<const KvUnit*>(a.plan + h.off_unit);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = a.G, kvh = a.kv_heads, H = G * kvh, M = h.M;
   const float2* pml = reinterpret_cast<const float2*>(a.part + (size_t)h.nslots * HD);
-  const bool split = h.split_rows != 0;
-  const int ks = split ? 4 : 1, k0 = split ? warp : 0;
-  const int head0 = split ? blockIdx.y : blockIdx.y * 4 + warp, heads = split ? gridDim.y : gridDim.y * 4;
-  for (int orow = blockIdx.x; orow < h.nseq * M; orow += gridDim.x) {
-    const int s = orow / M, t = orow - s * M;
+  constexpr int ks = SPLIT ? 4 : 1;
+  const int k0 = SPLIT ? warp : 0;
+  const int items = h.nseq * M * H, step = SPLIT ? gridDim.x : gridDim.x * 4;
+  for (int item = SPLIT ? blockIdx.x : blockIdx.x * 4 + warp; item < items; item += step) {
+    const int orow = item / H, head = item - orow * H, s = orow / M, t = orow - s * M;
     const KvSeq& q = sqs[s];
     if (t >= q.cnt) continue;
-    for (int head = head0; head < H; head += heads) {
-      const int g = head / G, row = q.row0 + t * G + (head - g * G);
-      // the partials of the row's ranges: entries [0, c0), [c0, c1), [c1, n); entry i in partial row b + i * d
-      int b[KV_LEVELS], d[KV_LEVELS], c[KV_LEVELS], n = 0;
+    const int g = head / G, row = q.row0 + t * G + (head - g * G);
+    // the partials of the row's ranges in order: entry i's slot, and how many there are
+    auto entry = [&](int i, int& n) {  // (not kept in registers for the few rows with more than 32)
+      int slot = 0;
+      n = 0;
 #pragma unroll
-      for (int l = 0; l < KV_LEVELS; l++) {
-        b[l] = d[l] = 0;
+      for (int l = 0; l < KV_LEVELS; l++)
         if (l < q.nlev) {
           const int lr = row - q.lrow0[l];
           const KvUnit u = units[q.lunit[l] + g * q.ltile[l] + lr / KV_TILE];
-          d[l] = u.nrows;
-          b[l] = u.base + lr % KV_TILE - n * u.nrows;
+          if (i >= n && i - n < u.nseg) slot = u.base + lr % KV_TILE + (i - n) * u.nrows;
           n += u.nseg;
         }
-        c[l] = n;
+      return slot;
+    };
+    // the warp's entries: k0, k0 + ks, .. ; lane i holds the weight of the i-th
+    int n, again;
+    int slot = entry(k0 + ks * lane, n);
+    n = (n - k0 + ks - 1) / ks;
+    pdl_wait();
+    const float2 none = make_float2(-CUDART_INF_F, 0.f);
+    float2 ml = lane < n ? pml[slot] : none;
+    const int flag = t > 0 ? a.flags[s * kvh + g] : 0;
+    V v[U];
+    auto load = [&](int k) {  // entries k .. k + U of the 32 whose slots the lanes hold
+#pragma unroll
+      for (int e = 0; e < U; e++) {
+        const int sl = __shfl_sync(0xffffffffu, slot, (k + e) & 31);
+        if (k + e < n) v[e] = *reinterpret_cast<const V*>(a.part + (size_t)sl * HD + lane * W);
       }
-      auto slot_of = [&](int i) { return i < c[0] ? b[0] + i * d[0] : i < c[1] ? b[1] + i * d[1] : b[2] + i * d[2]; };
-      pdl_wait();
-      const float2 none = make_float2(-CUDART_INF_F, 0.f);
-      int slot = slot_of(lane);  // of the entry whose weight this lane holds
-      float2 ml = lane < n ? pml[slot] : none;
-      const int flag = t > 0 ? a.flags[s * kvh + g] : 0;
-      V v[4];
-      auto load = [&](int k) {  // entries k, k + ks, .. of the 32 whose slots the lanes hold
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int sl = __shfl_sync(0xffffffffu, slot, (k + e * ks) & 31);
-          if (k + e * ks < n) v[e] = *reinterpret_cast<const V*>(a.part + (size_t)sl * HD + lane * W);
-        }
-      };
-      load(k0);
-      float m = ml.x;
+    };
+    load(0);
+    float m = ml.x;
 #pragma unroll 1
-      for (int i = 32 + lane; i < n; i += 32) m = fmaxf(m, pml[slot_of(i)].x);
-      m = warp_max(m);
-      float l = 0.f, acc[W];
+    for (int i = 32 + lane; i < n; i += 32) m = fmaxf(m, pml[entry(k0 + ks * i, again)].x);
+    m = warp_max(m);
+    float l = 0.f, acc[W];
 #pragma unroll
-      for (int e = 0; e < W; e++) acc[e] = 0.f;
+    for (int e = 0; e < W; e++) acc[e] = 0.f;
 #pragma unroll 1
-      for (int base = 0; base < n; base += 32) {
-        if (base > 0) {
-          slot = slot_of(base + lane);
-          ml = base + lane < n ? pml[slot] : none;
-        }
-        const float w = ml.x == -CUDART_INF_F ? 0.f : kv_ex2(ml.x - m);
-        l += w * ml.y;
+    for (int base = 0; base < n; base += 32) {
+      if (base > 0) {
+        slot = entry(k0 + ks * (base + lane), again);
+        ml = base + lane < n ? pml[slot] : none;
+      }
+      const float w = ml.x == -CUDART_INF_F ? 0.f : kv_ex2(ml.x - m);
+      l += w * ml.y;
 #pragma unroll 1
-        for (int k = base + k0; k < min(n, base + 32); k += 4 * ks) {
-          if (k > k0) load(k);
+      for (int k = base; k < min(n, base + 32); k += U) {
+        if (k > 0) load(k);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float wk = __shfl_sync(0xffffffffu, w, (k + e * ks) & 31);
-            if (k + e * ks < n) {
-              const float* f = reinterpret_cast<const float*>(&v[e]);
+        for (int e = 0; e < U; e++) {
+          const float wk = __shfl_sync(0xffffffffu, w, (k + e) & 31);
+          if (k + e < n) {
+            const float* f = reinterpret_cast<const float*>(&v[e]);
 #pragma unroll
-              for (int x = 0; x < W; x++) acc[x] += wk * f[x];
-            }
+            for (int x = 0; x < W; x++) acc[x] += wk * f[x];
           }
         }
       }
-      l = warp_sum(l);
-      if (split) {
-        __syncthreads();  // (the last row's sums have been read)
-        *reinterpret_cast<V*>(&s_acc[warp][lane * W]) = *reinterpret_cast<V*>(acc);
-        __syncthreads();
-        if (warp != 0) continue;
-#pragma unroll
-        for (int x = 0; x < W; x++) acc[x] = (s_acc[0][lane * W + x] + s_acc[1][lane * W + x]) + (s_acc[2][lane * W + x] + s_acc[3][lane * W + x]);
-      }
-      const float inv = 1.0f / l;
-#pragma unroll
-      for (int e = 0; e < W; e++) acc[e] *= inv;
-      if (flag) {  // infinities and NaN of the block's own V rows that this row sees
-#pragma unroll 1
-        for (int tt = 1; tt <= t; tt++) {
-          const int pos = q.n + tt;
-          const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * W;
-#pragma unroll
-          for (int e = 0; e < W; e += 2) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(a.v + src + e);
-            const uint32_t nf = kv_nonfinite<BF16>(x);
-            const float2 f = kv_unpack<BF16>(x);
-            if (nf & 0xffffu) acc[e] += f.x;
-            if (nf >> 16) acc[e + 1] += f.y;
-          }
-        }
-      }
-      uint16_t* out = BT ? a.out + bt_off(orow, head * HD + lane * W, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * W;
-      if constexpr (W == 4)
-        *reinterpret_cast<uint2*>(out) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
-      else
-        *reinterpret_cast<uint32_t*>(out) = kv_pack<BF16>(acc[0], acc[1]);
     }
+    l = warp_sum(l);
+    if constexpr (SPLIT) {
+      __syncthreads();  // (the last row's sums have been read)
+      *reinterpret_cast<V*>(&s_acc[warp][lane * W]) = *reinterpret_cast<V*>(acc);
+      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      __syncthreads();
+      if (warp != 0) continue;
+      m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
+      l = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; x++) acc[x] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float w = s_ml[e].x == -CUDART_INF_F ? 0.f : kv_ex2(s_ml[e].x - m);
+        l += w * s_ml[e].y;
+#pragma unroll
+        for (int x = 0; x < W; x++) acc[x] += w * s_acc[e][lane * W + x];
+      }
+    }
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < W; e++) acc[e] *= inv;
+    if (flag) {  // infinities and NaN of the block's own V rows that this row sees
+#pragma unroll 1
+      for (int tt = 1; tt <= t; tt++) {
+        const int pos = q.n + tt;
+        const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * W;
+#pragma unroll
+        for (int e = 0; e < W; e += 2) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(a.v + src + e);
+          const uint32_t nf = kv_nonfinite<BF16>(x);
+          const float2 f = kv_unpack<BF16>(x);
+          if (nf & 0xffffu) acc[e] += f.x;
+          if (nf >> 16) acc[e + 1] += f.y;
+        }
+      }
+    }
+    uint16_t* out = BT ? a.out + bt_off(orow, head * HD + lane * W, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * W;
+    if constexpr (W == 4)
+      *reinterpret_cast<uint2*>(out) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
+    else
+      *reinterpret_cast<uint32_t*>(out) = kv_pack<BF16>(acc[0], acc[1]);
   }
+}
+template <int HD, bool BF16, bool BT>
+__global__ void __launch_bounds__(128, 8) kv_merge_kernel(const KvArgs a) {
+  __shared__ __align__(16) float s_acc[4][HD];
+  __shared__ float2 s_ml[4];
+  pdl_trigger();
+  if (reinterpret_cast<const KvHdr*>(a.plan)->split_rows)
+    kv_merge<HD, BF16, BT, true>(a, s_acc, s_ml);
+  else
+    kv_merge<HD, BF16, BT, false>(a, s_acc, s_ml);
   pdl_wait();  // (a warp without rows: the kernel after this one may rely on the one before it being done)
 }
 
@@ -1021,8 +1044,8 @@ void KvWork::close() {
 template <int HD, bool BF16>
 static void launch_kv_t(const KvWork& w, const KvAttn& a, const KvArgs& k, cudaStream_t s) {
   const int units = (w.g.heads + 2 * w.g.kv_heads) * (HD / 16);
-  const size_t items = (size_t)a.rows * units;
-  const int gp = (int)std::min<size_t>((items + 255) / 256, (size_t)w.g.nctas * 8);
+  const size_t pieces = (size_t)a.rows * units;
+  const int gp = (int)std::min<size_t>((pieces + 255) / 256, (size_t)w.g.nctas * 8);
   if (a.qkv_f32)
     launch_pdl(kv_prep_kernel<BF16, true>, dim3(gp), dim3(256), 0, s, k);
   else
@@ -1030,12 +1053,13 @@ static void launch_kv_t(const KvWork& w, const KvAttn& a, const KvArgs& k, cudaS
   const size_t smem = KvSmem<HD>::kTotal;
   ensure_smem(kv_attn_kernel<HD, BF16>, smem);
   launch_pdl(kv_attn_kernel<HD, BF16>, dim3(w.g.nctas), dim3(KV_THREADS), smem, s, k, w.qmap, w.qmap_half, *a.kmap, *a.vmap);
-  // a block per row, the heads over grid.y as far as it takes to fill the GPU
-  const int gr = std::min(a.rows, w.g.nctas * 16), gh = std::min(w.g.heads, std::max((w.g.heads + 15) / 16, (w.g.nctas * 8 + gr - 1) / gr));
+  // a warp per row and head, or a block for each of as many as the plan may split
+  const size_t items = (size_t)a.rows * w.g.heads;
+  const int gm = (int)std::min(std::max((items + 3) / 4, std::min(items, (size_t)w.g.nctas * KV_SPLIT_ITEMS)), (size_t)w.g.nctas * 16);
   if constexpr (!BF16) {
-    if (a.out_bt) return launch_pdl(kv_merge_kernel<HD, false, true>, dim3(gr, gh), dim3(128), 0, s, k);
+    if (a.out_bt) return launch_pdl(kv_merge_kernel<HD, false, true>, dim3(gm), dim3(128), 0, s, k);
   }
-  launch_pdl(kv_merge_kernel<HD, BF16, false>, dim3(gr, gh), dim3(128), 0, s, k);
+  launch_pdl(kv_merge_kernel<HD, BF16, false>, dim3(gm), dim3(128), 0, s, k);
 }
 
 void launch_kv_attention(const KvWork& w, const KvAttn& a, cudaStream_t s) {

@@ -44,6 +44,7 @@ void launch_stage(int32_t* table, const KvRange* ranges, int nranges, void* plan
 
 constexpr int KV_TILE = 128;    // query rows of a tile
 constexpr int KV_CHUNK = 128;   // positions of a chunk
+constexpr int KV_SPLIT_ITEMS = 8;  // rows x heads per CTA up to which the merge may take four warps for each
 constexpr int KV_LEVELS = 3;    // nodes on a row's path: two shared ranges at most, then its own
 
 struct KvSeg {
@@ -82,7 +83,7 @@ struct KvUnit {     // a tile's partials: segment k's of its row r in partial ro
 struct KvHdr {
   int32_t M, nseq, R, max_pages;  // R: rows of a kv head's query operand
   int32_t off_prog, off_seg, off_seq, off_unit;  // byte offsets in the plan
-  int32_t nslots, split_rows;  // split_rows: some row has many partials (kv_merge_kernel)
+  int32_t nslots, split_rows;  // split_rows: few rows, some with many partials (kv_merge_kernel)
   int32_t pad[2];
 };
 

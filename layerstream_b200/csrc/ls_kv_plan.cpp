@@ -16,12 +16,15 @@ constexpr long long kMinSaved = 256;
 
 // Time of a CTA's work in units of one pair chunk: a chunk for two tiles, for one tile (the two lanes work on
 // different ones), and what a piece costs before its first chunk and after its last. From timelines of the CTAs
-// (hd 64 and 128, 2 to 64 readers of 2k to 64k positions): a pair chunk takes 3400 and 4200 cycles. With the starts
-// left out the CTAs of single tiles ended 40 % after those of pairs, with these all end within 20 % of the mean
-// (four prompts of 8k with 16 samples each 61.8 against 54.8 us, a prefill of eight chunks 52.8 against 46.5).
-constexpr double kPairChunk = 1.0, kSingleChunk = 0.55, kPairStart = 1.5, kSingleStart = 0.4;
+// (hd 64 and 128, 2 to 64 readers of 2k to 64k positions): a pair chunk takes about 3400 cycles. With the starts of
+// pieces that a CTA's end cuts left out, the CTAs of single tiles ended 40 % after those of pairs; with these
+// all end within 15 % of the mean (four prompts of 8k with 16 samples each 61.8 against 54.8 us, a prefill of
+// eight chunks 52.8 against 46.5). A single chunk at 0.55 instead: 64 readers of 32k 68.6 against 65.4 us.
+constexpr double kPairChunk = 1.0, kSingleChunk = 0.62, kPairStart = 1.5, kSingleStart = 0.4;
 
-// A row with more partials than this is merged by four warps instead of one.
+// A row with more partials than this is merged by four warps instead of one when rows and heads are few
+// (KV_SPLIT_ITEMS). 16 rows of 14 heads, 40 partials: one warp 10.4 us, four 5.6; 288 rows of 16 heads, 10
+// partials: 7.0 and 13.3.
 constexpr int kSplitRows = 8;
 
 static size_t align16(size_t n) { return (n + 15) / 16 * 16; }
@@ -293,7 +296,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   h.R = R;
   h.max_pages = g.max_pages;
   h.nslots = slots;
-  h.split_rows = most > kSplitRows;
+  h.split_rows = most > kSplitRows && (long long)R * kvh <= (long long)g.nctas * KV_SPLIT_ITEMS;
   size_t at = align16(sizeof(KvHdr));
   auto place = [&](int32_t& off, size_t n) {
     off = (int32_t)at;
