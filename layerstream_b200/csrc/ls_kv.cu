@@ -257,7 +257,7 @@ struct KvArgs {
   int* err;
   uint16_t* out;
   size_t qkv_stride, out_stride;
-  int G, kv_heads, hd, shift, num_pages, out_bt_n;
+  int G, kv_heads, hd, shift, num_pages, out_bt_n, rows, M;
 };
 
 // One thread per 16 elements of a row: dims [8 i, 8 i + 8) and their rotation partners hd / 2 further
@@ -269,49 +269,44 @@ __global__ void __launch_bounds__(256) kv_prep_kernel(const KvArgs a) {
   pdl_wait();
   pdl_trigger();
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
-  const KvSeq* sq = reinterpret_cast<const KvSeq*>(a.plan + h.off_seq);
+  const KvSeq* sq = reinterpret_cast<const KvSeq*>(a.plan + KV_SEQ_AT);
   const int G = a.G, kvh = a.kv_heads, H = G * kvh, hd = a.hd, half = hd / 2, per = hd / 16;
   const int units = (H + 2 * kvh) * per;
-  const int M = h.M;
-  const size_t total = (size_t)h.nseq * M * units;
+  const size_t total = (size_t)a.rows * units;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
     const int row = (int)(i / units), u = (int)(i - (size_t)row * units);
-    const int s = row / M, t = row - s * M;
-    const KvSeq q = sq[s];
-    if (t >= q.cnt) continue;
+    const int s = row / a.M, t = row - s * a.M;
+    const int4 q4 = *reinterpret_cast<const int4*>(sq + s);  // the first fields, in one load
+    const int n = q4.x, cnt = q4.y, row0 = q4.z, tab = q4.w, pos = n + t;
+    if (t >= cnt) continue;
     const int head = u / per, c = u - head * per;
     const size_t src = (size_t)row * a.qkv_stride + (size_t)head * hd;
-    const int pos = q.n + t;
+    const bool rot = head < H + kvh;
     float x[8], y[8];
-    if (head < H + kvh) {
-      kv_load8<BF16, F32>(a.qkv, src + c * 8, x);
-      kv_load8<BF16, F32>(a.qkv, src + half + c * 8, y);
-      if (a.rope) {
-        const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * half + c * 8);
+    kv_load8<BF16, F32>(a.qkv, src + c * (rot ? 8 : 16), x);
+    kv_load8<BF16, F32>(a.qkv, src + (rot ? half + c * 8 : c * 16 + 8), y);
+    if (rot && a.rope) {
+      const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * half + c * 8);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float4 w = cs[e];
-          const float x0 = x[2 * e], y0 = y[2 * e], x1 = x[2 * e + 1], y1 = y[2 * e + 1];
-          x[2 * e] = x0 * w.x - y0 * w.y;
-          y[2 * e] = y0 * w.x + x0 * w.y;
-          x[2 * e + 1] = x1 * w.z - y1 * w.w;
-          y[2 * e + 1] = y1 * w.z + x1 * w.w;
-        }
+      for (int e = 0; e < 4; e++) {
+        const float4 w = cs[e];
+        const float x0 = x[2 * e], y0 = y[2 * e], x1 = x[2 * e + 1], y1 = y[2 * e + 1];
+        x[2 * e] = x0 * w.x - y0 * w.y;
+        y[2 * e] = y0 * w.x + x0 * w.y;
+        x[2 * e + 1] = x1 * w.z - y1 * w.w;
+        y[2 * e + 1] = y1 * w.z + x1 * w.w;
       }
-    } else {
-      kv_load8<BF16, F32>(a.qkv, src + c * 16, x);
-      kv_load8<BF16, F32>(a.qkv, src + c * 16 + 8, y);
     }
     const uint4 xv = kv_pack8<BF16>(x), yv = kv_pack8<BF16>(y);
     if (head < H) {
       const int g = head / G, j = head - g * G;
-      uint16_t* d = a.q + ((size_t)g * h.R + q.row0 + (size_t)t * G + j) * hd + c * 8;
+      uint16_t* d = a.q + ((size_t)g * h.R + row0 + (size_t)t * G + j) * hd + c * 8;
       *reinterpret_cast<uint4*>(d) = xv;
       *reinterpret_cast<uint4*>(d + half) = yv;
     } else {
       const bool is_v = head >= H + kvh;
       const int g = head - H - (is_v ? kvh : 0);
-      const int page = a.tables[q.tab + (pos >> a.shift)];
+      const int page = a.tables[tab + (pos >> a.shift)];
       const size_t dst = ((((size_t)g * a.num_pages + page) << a.shift) + (pos & ((1 << a.shift) - 1))) * hd;
       if (is_v) {
         *reinterpret_cast<uint4*>(a.v + dst + c * 16) = xv;
@@ -386,8 +381,6 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = s_tmem;
-  pdl_wait();  // the query operand and the block's K/V rows
-
   // Ring use of lane t's chunk: pair chunk i is in stage i % NS of K and of V; chunk j of a lane's own
   // phase in stage (2 j + t) % NS, so that each lane's own stages advance with that lane alone. Its
   // phase is the number of uses the stage had before.
@@ -404,7 +397,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
       int seg, end, j, chunk;
     };
     Cursor c = {0, pr.nseg[0], 0, 0}, other = {pr.npair, pr.nseg[1], 0, pr.pair_ch};  // of lane t, of the other lane
-    bool ok = true;
+    bool ok = true, waited = false;
     uint32_t issued = 0, parity = 0;  // per ring slot (K stages, then V stages): a copy was issued, its phase's parity
     int t = 0;
     auto swap = [&] {
@@ -416,6 +409,10 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     while (ok && (c.seg < c.end || other.seg < other.end)) {
       if (c.seg >= c.end) swap();
       const KvSeg& s = seg_of(t, c.seg);
+      if (!waited && s.causal != INT_MAX) {  // the block's own K/V rows; what was cached before is there already
+        pdl_wait();
+        waited = true;
+      }
       const int pc = s.p0 + c.j * KV_CHUNK;
       const int npg = (min(KV_CHUNK, s.p1 - pc) + pg_rows - 1) / pg_rows;
       const int i = lane / CB, cb = lane - i * CB;
@@ -453,6 +450,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   } else if (warp >= 8) {
     // ---- MMA issuer of lane t (the whole warp runs it, one lane issues) ----
     const int t = warp - 8, nseg = pr.nseg[t];
+    pdl_wait();  // the query operand
     if (nseg > 0) {
       const uint32_t lead = kv_elect();
       const uint32_t sq = smem + SM::kQ + t * SM::kTile;
@@ -584,6 +582,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
     }
   } else {
     // ---- softmax of lane t: one query row per thread ----
+    pdl_wait();  // the sequences' flags, cleared
     const int t = warp >> 2, quad = warp & 3;
     const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t t_o = at + COL_O + t * HD;
@@ -767,14 +766,14 @@ __device__ __forceinline__ void kv_merge(const KvArgs& a, float (*s_acc)[HD], fl
   constexpr int W = HD / 32, U = 4;  // f32 per lane, partials in flight
   using V = std::conditional_t<W == 4, float4, float2>;
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
-  const KvSeq* sqs = reinterpret_cast<const KvSeq*>(a.plan + h.off_seq);
+  const KvSeq* sqs = reinterpret_cast<const KvSeq*>(a.plan + KV_SEQ_AT);
   const KvUnit* units = reinterpret_cast<const KvUnit*>(a.plan + h.off_unit);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = a.G, kvh = a.kv_heads, H = G * kvh, M = h.M;
+  const int G = a.G, kvh = a.kv_heads, H = G * kvh, M = a.M;
   const float2* pml = reinterpret_cast<const float2*>(a.part + (size_t)h.nslots * HD);
   constexpr int ks = SPLIT ? 4 : 1;
   const int k0 = SPLIT ? warp : 0;
-  const int items = h.nseq * M * H, step = SPLIT ? gridDim.x : gridDim.x * 4;
+  const int items = a.rows * H, step = SPLIT ? gridDim.x : gridDim.x * 4;
   for (int item = SPLIT ? blockIdx.x : blockIdx.x * 4 + warp; item < items; item += step) {
     const int orow = item / H, head = item - orow * H, s = orow / M, t = orow - s * M;
     const KvSeq& q = sqs[s];
@@ -1083,6 +1082,8 @@ void launch_kv_attention(const KvWork& w, const KvAttn& a, cudaStream_t s) {
   k.shift = w.g.shift;
   k.num_pages = w.g.num_pages;
   k.out_bt_n = a.out_bt_n;
+  k.rows = a.rows;
+  k.M = a.M;
   if (w.g.hd == 64) return w.bf16 ? launch_kv_t<64, true>(w, a, k, s) : launch_kv_t<64, false>(w, a, k, s);
   return w.bf16 ? launch_kv_t<128, true>(w, a, k, s) : launch_kv_t<128, false>(w, a, k, s);
 }

@@ -82,10 +82,12 @@ struct KvUnit {     // a tile's partials: segment k's of its row r in partial ro
 };
 struct KvHdr {
   int32_t M, nseq, R, max_pages;  // R: rows of a kv head's query operand
-  int32_t off_prog, off_seg, off_seq, off_unit;  // byte offsets in the plan
+  int32_t off_prog, off_seg, off_unit;  // byte offsets in the plan (the sequences stand at KV_SEQ_AT)
   int32_t nslots, split_rows;  // split_rows: few rows, some with many partials (kv_merge_kernel)
-  int32_t pad[2];
+  int32_t pad[3];
 };
+constexpr int KV_SEQ_AT = sizeof(KvHdr);  // where the plan's sequences stand: read without the header
+static_assert(KV_SEQ_AT % 16 == 0, "plan sections start on 16 bytes");
 
 struct KvGeom {
   int heads = 0, kv_heads = 0, hd = 0, shift = 6, num_pages = 0, max_pages = 0, nseq = 0, max_rows = 0, nctas = 148;
@@ -176,7 +178,7 @@ struct KvAttn {
   size_t out_stride = 0;
   uint16_t* out_bt = nullptr; // instead of out: f16 in the batched GEMM's operand layout (groups of out_bt_n rows)
   int out_bt_n = 0;
-  int rows = 0;               // nseq * M
+  int rows = 0, M = 0;        // nseq * M, rows of a sequence
 };
 void launch_kv_attention(const KvWork& w, const KvAttn& a, cudaStream_t s);
 // 2-D tensor map over rows of hd 16-bit elements (64 x box_rows boxes, 128-byte swizzle).

@@ -417,7 +417,8 @@ struct LsKv {
     a.vmap = &maps[2 * layer + 1];
     a.out = out;
     a.out_stride = out_stride;
-    a.rows = reinterpret_cast<const KvHdr*>(planner.bytes.data())->M * g.nseq;
+    a.M = reinterpret_cast<const KvHdr*>(planner.bytes.data())->M;
+    a.rows = a.M * g.nseq;
     launch_kv_attention(work, a, st);
   }
 

@@ -297,14 +297,13 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   h.max_pages = g.max_pages;
   h.nslots = slots;
   h.split_rows = most > kSplitRows && (long long)R * kvh <= (long long)g.nctas * KV_SPLIT_ITEMS;
-  size_t at = align16(sizeof(KvHdr));
+  size_t at = KV_SEQ_AT + align16(dseqs_.size() * sizeof(KvSeq));
   auto place = [&](int32_t& off, size_t n) {
     off = (int32_t)at;
     at += align16(n);
   };
   place(h.off_prog, progs_.size() * sizeof(KvProg));
   place(h.off_seg, segs_.size() * sizeof(KvSeg));
-  place(h.off_seq, dseqs_.size() * sizeof(KvSeq));
   place(h.off_unit, units_.size() * sizeof(KvUnit));
   bytes.resize(at);
   auto put = [&](int32_t off, const void* p, size_t n) {
@@ -313,7 +312,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   put(0, &h, sizeof h);
   put(h.off_prog, progs_.data(), progs_.size() * sizeof(KvProg));
   put(h.off_seg, segs_.data(), segs_.size() * sizeof(KvSeg));
-  put(h.off_seq, dseqs_.data(), dseqs_.size() * sizeof(KvSeq));
+  put(KV_SEQ_AT, dseqs_.data(), dseqs_.size() * sizeof(KvSeq));
   put(h.off_unit, units_.data(), units_.size() * sizeof(KvUnit));
   if (at > g.plan_cap()) LS_THROW(LS_ERR_ARG, "internal: an attention plan outgrew its workspace");
 }
@@ -327,7 +326,7 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(bytes.data());
   const auto* prog = reinterpret_cast<const KvProg*>(bytes.data() + h.off_prog);
   const auto* seg = reinterpret_cast<const KvSeg*>(bytes.data() + h.off_seg);
-  const auto* sq = reinterpret_cast<const KvSeq*>(bytes.data() + h.off_seq);
+  const auto* sq = reinterpret_cast<const KvSeq*>(bytes.data() + KV_SEQ_AT);
   const auto* unit = reinterpret_cast<const KvUnit*>(bytes.data() + h.off_unit);
   const int G = g.G();
   need((size_t)h.R <= g.rows_cap() && (size_t)h.nslots <= g.slots_cap() && h.nseq == (int)seqs.size(), "header");

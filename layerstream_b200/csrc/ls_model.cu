@@ -2275,6 +2275,7 @@ struct LsBatch {
         k.out_bt = a.out_h;
         k.out_bt_n = a.out_h_n;
         k.rows = (int)T;
+        k.M = M;
         launch_kv_attention(kvw, k, stream);
       } else {
         launch_attention(a, stream);
