@@ -674,12 +674,15 @@ class KvCache:
 def kv_copy_pages(k_ptr: int, v_ptr: int, layers: int, kv_heads: int, hd: int, page: int, num_pages: int, src, dst, rows=None,
                   stream: int = 0):
     """Rows [0, rows[i]) (None: whole pages) of page src[i] to page dst[i], in every layer and kv head of both pools."""
-    s, d = np.array(src, np.int32), np.array(dst, np.int32)
-    r = None if rows is None else np.array(rows, np.int32)
-    if s.ndim != 1 or s.shape != d.shape or (r is not None and r.shape != s.shape):
+    try:
+        lists = np.array((src, dst) if rows is None else (src, dst, rows), np.int32)  # (one array: small calls are host-bound)
+    except ValueError:
+        lists = None
+    if lists is None or lists.ndim != 2:
         raise ValueError("src, dst and rows must have the same length")
-    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, _addr(s), _addr(d), None if r is None else _addr(r),
-                                  s.size, stream))
+    n, at = lists.shape[1], _addr(lists)
+    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, at, at + 4 * n, None if rows is None else at + 8 * n,
+                                  n, stream))
 
 
 def qgemv_rows_noalloc(bits: int, group: int, rows_ptr: int, rows: int, cols: int, x_ptr: int, M: int, y_ptr: int,

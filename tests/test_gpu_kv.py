@@ -408,3 +408,96 @@ def test_refusals_with_a_gpu():
                    max_rows=4)
     with pytest.raises(ls.LayerstreamError, match="device memory"):
         ls.kv_copy_pages(host.ctypes.data & ~15, s.v.data_ptr(), 1, 2, 64, 16, 4, [0], [1])
+
+
+@pytest.mark.parametrize("heads,kvh,hd,dtype,seqs,M,prefix,tail", [
+    (2, 1, 64, "f16", 1, 1, 40000, 0),     # one row over all CTAs: the join's four warps hold more than 32 partials each
+    (2, 1, 128, "bf16", 1, 3, 20000, 0),
+    (15, 1, 64, "bf16", 4, 20, 33000, 30),  # many rows of few tiles: one warp joins about 30 partials
+])
+def test_long_contexts(heads, kvh, hd, dtype, seqs, M, prefix, tail):
+    s = Setup(heads, kvh, hd, dtype, 64, seqs, M, prefix + tail * seqs + M, seed=11)
+    shared = list(range(prefix // 64))
+    at = len(shared)
+    for i in range(seqs):
+        n = prefix // 64 * 64 + tail * (i + 1)
+        own = -(-n // 64) - len(shared)
+        s.fill_fast(i, shared + list(range(at, at + own)), n)
+        at += own
+    s.kv.begin([M] * seqs, M)
+    run_layer(s, 0, [M] * seqs)
+
+
+@pytest.mark.parametrize("hd,dtype,n", [(64, "f16", 500), (128, "bf16", 700), (128, "f16", 1000)])
+def test_a_row_does_not_depend_on_its_neighbours(hd, dtype, n):
+    # NaN, and scores that outgrow the running maximum, in one row of a tile: the others keep every bit
+    M = 8
+    s = Setup(8, 2, hd, dtype, 32, 2, M, n + M, seed=5)
+    pages = list(range(-(-n // 32)))
+    s.fill_fast(0, pages, n)
+    s.kv.fork(0, [1])
+    s.kv.begin([M, M], M)
+    qkv = s.randn(2 * M, s.W)
+    clean = run_layer(s, 0, [M, M], qkv, check=False).view(2, M, 8, hd)
+    big = qkv.clone()
+    big[2, : 8 * hd] *= 30
+    big[M + 5, hd: 2 * hd] = math.nan
+    got = run_layer(s, 0, [M, M], big, check=False).view(2, M, 8, hd)
+    assert torch.isnan(got[1, 5, 1]).all()
+    same = torch.ones(2, M, 8, dtype=torch.bool, device="cuda")
+    same[0, 2] = False
+    same[1, 5, 1] = False
+    assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, "f16"), (128, "bf16")])
+def test_an_infinite_key(hd, dtype):
+    # its score is +inf for the rows that are NaN by the definition too, -inf (weight 0) for the others
+    s = Setup(4, 2, hd, dtype, 16, 2, 2, 330, seed=9)
+    s.fill_fast(0, list(range(20)), 300)
+    s.k[0, 0, 3, 5, 7] = math.inf
+    s.kv.fork(0, [1])
+    s.kv.begin([2, 2], 2)
+    lens, tables = [300, 300], s.kv.tables()
+    qkv = s.randn(4, s.W)
+    got = run_layer(s, 0, [2, 2], qkv, rope=False, check=False)
+    qz = qkv.view(4, -1, hd)[:, :2, 7].float()  # kv head 0's q heads: sign of q . k
+    nan = qz > 0
+    out = got.view(4, 4, hd)
+    assert torch.isnan(out[:, :2][nan]).all() and torch.isfinite(out[:, 2:]).all() and torch.isfinite(out[:, :2][~nan]).all()
+    at = torch.arange(302, device="cuda")
+    for i in range(2):
+        pg = torch.as_tensor(tables[i].astype(np.int64), device="cuda")[at // 16]
+        K, V = s.k[0][0, pg, at % 16].double(), s.v[0][0, pg, at % 16].double()
+        for t in range(2):
+            e = lens[i] + t + 1
+            seen = torch.ones(e, dtype=torch.bool, device="cuda")
+            seen[3 * 16 + 5] = False
+            for j in range(2):
+                if nan[2 * i + t, j]:
+                    continue
+                q = qkv[2 * i + t].view(-1, hd)[j].double()
+                p = torch.softmax(K[:e][seen] @ q / math.sqrt(hd), 0)
+                o, a = p @ V[:e][seen], p @ V[:e][seen].abs()
+                d = s.u * ((K[:e][seen].abs() @ q.abs()) / math.sqrt(hd)).max()
+                tiny = e * 2.0**-25 * V[:e].abs().amax() if s.dt == torch.float16 else 0.0
+                assert ((out[2 * i + t, j].double() - o).abs() <= s.u * o.abs() + (s.u + torch.expm1(2 * d) + 2**-14) * a + tiny + 1e-7).all()
+
+
+def test_two_caches_on_two_streams():
+    setups = [Setup(8, 2, 64, "f16", 16, 4, 3, 900, seed=21), Setup(4, 2, 128, "bf16", 32, 6, 2, 1500, seed=22)]
+    streams, qkvs, alone = [torch.cuda.Stream() for _ in setups], [], []
+    for s, n in zip(setups, (800, 1400)):
+        s.fill_fast(0, list(range(-(-n // s.page))), n)
+        s.kv.fork(0, range(1, s.seqs))
+        s.kv.begin([s.M] * s.seqs, s.M)
+        qkvs.append(s.randn(s.seqs * s.M, s.W))
+        alone.append(run_layer(s, 0, [s.M] * s.seqs, qkvs[-1]))
+    outs = [torch.zeros_like(a) for a in alone]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, st, q, o in zip(setups, streams, qkvs, outs):
+            s.kv.attention(0, q.data_ptr(), o.data_ptr(), s.rope.data_ptr(), stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert torch.equal(a, o)
