@@ -287,7 +287,7 @@ int ls_batch_tp_peer(const LsBatch *b, int *on);
  * not overlap (the caller orders the streams). ls_kv_begin and ls_kv_compact are refused on a stream
  * that is being captured; ls_kv_attention may be captured, and a replay runs the plan of the step that is
  * begun then: it is valid between ls_kv_begin and ls_kv_end of a step with the M it was captured at,
- * over the same qkv, rope and out buffers. Replays on one cache must not overlap either. */
+ * over the same qkv, rope and out buffers, until the cache is freed. Replays on one cache must not overlap either. */
 typedef struct LsKv LsKv;
 #define LS_KV_F16 0
 #define LS_KV_BF16 1
