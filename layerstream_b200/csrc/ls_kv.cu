@@ -756,33 +756,35 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
 // ---- the partials ---------------------------------------------------------------------------------
 
 // A query row's partials: their maximum, then their weighted sum, in plan order (the result does not
-// depend on timing). One warp per row and head, or, when the plan says so (few rows, some with many
-// partials), the block's four warps, each with every fourth of them (SPLIT). Bound by L2's latency when there
-// are few rows (sequence, units, then the maxima and four partials at once: three round trips, 3.5 us), by
-// L2's bandwidth when there are many (4608 rows with 10 partials of 512 bytes: 6.8 us). Eight partials in
-// flight take registers, and so warps, away: 288 rows of 16 heads 9.0 against 8.2 us, 1024 rows of
-// 14 heads 12.1 against 10.8; so does a kernel not held to 64 registers (22.1 against 23.4 us for the three
-// launches at 4608 rows). BT: f16 in the batched GEMM's operand layout.
+// depend on timing). A group of hd / 4 threads per row and head, 16 bytes of a partial each, or, when the plan
+// says so (few rows, some with many partials), the block's groups together, each with every NG-th of them
+// (SPLIT). Bound by L2's latency when there are few rows (sequence, units, then the maxima and four
+// partials at once: three round trips, 3.7 us), by L2's bandwidth when there are many (4608 rows with 10
+// partials of 512 bytes: 6.5 us). A whole warp per row at hd 64 too: 14.5 against 9.5 us for 64 x 32 rows
+// of 14 heads. Eight partials in flight take registers, and so warps, away: 288 rows of 16 heads 9.0 against
+// 8.2 us, 1024 rows of 14 heads 12.1 against 10.8; so does a kernel not held to 64 registers (22.1
+// against 23.4 us for the three launches at 4608 rows). BT: f16 in the batched GEMM's operand layout.
 template <int HD, bool BF16, bool BT, bool SPLIT>
 __device__ __forceinline__ void kv_merge(const KvArgs& a, float (*s_acc)[HD], float2* s_ml) {
-  constexpr int W = HD / 32, U = 4;  // f32 per lane, partials in flight
-  using V = std::conditional_t<W == 4, float4, float2>;
-  const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
+  constexpr int L = HD / 4, NG = 128 / L, PER = 32 / L, U = 4;  // lanes of a group, groups of a block and a warp; partials in flight
   const KvSeq* sqs = reinterpret_cast<const KvSeq*>(a.plan + KV_SEQ_AT);
+  const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvUnit* units = reinterpret_cast<const KvUnit*>(a.plan + h.off_unit);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L, warp = threadIdx.x >> 5;
   const int G = a.G, kvh = a.kv_heads, H = G * kvh, M = a.M;
   const float2* pml = reinterpret_cast<const float2*>(a.part + (size_t)h.nslots * HD);
-  constexpr int ks = SPLIT ? 4 : 1;
-  const int k0 = SPLIT ? warp : 0;
-  const int items = a.rows * H, step = SPLIT ? gridDim.x : gridDim.x * 4;
-  for (int item = SPLIT ? blockIdx.x : blockIdx.x * 4 + warp; item < items; item += step) {
+  constexpr int ks = SPLIT ? NG : 1;
+  const int k0 = SPLIT ? grp : 0, sub = SPLIT ? 0 : grp % PER;
+  const int items = a.rows * H, step = SPLIT ? gridDim.x : gridDim.x * NG;
+  for (int it = SPLIT ? blockIdx.x : blockIdx.x * NG + warp * PER; it < items; it += step) {
+    const int item = min(it + sub, items - 1);
     const int orow = item / H, head = item - orow * H, s = orow / M, t = orow - s * M;
     const KvSeq& q = sqs[s];
-    if (t >= q.cnt) continue;
+    const bool valid = it + sub < items && t < q.cnt;
+    if ((SPLIT || PER == 1) && !valid) continue;  // (the groups of a warp stay together)
     const int g = head / G, row = q.row0 + t * G + (head - g * G);
     // the partials of the row's ranges in order: entry i's slot, and how many there are
-    auto entry = [&](int i, int& n) {  // (not kept in registers for the few rows with more than 32)
+    auto entry = [&](int i, int& n) {  // (not kept in registers for the few rows with more than L)
       int slot = 0;
       n = 0;
 #pragma unroll
@@ -795,81 +797,86 @@ __device__ __forceinline__ void kv_merge(const KvArgs& a, float (*s_acc)[HD], fl
         }
       return slot;
     };
-    // the warp's entries: k0, k0 + ks, .. ; lane i holds the weight of the i-th
-    int n, again;
-    int slot = entry(k0 + ks * lane, n);
-    n = (n - k0 + ks - 1) / ks;
+    // the group's entries: k0, k0 + ks, .. ; lane i holds the weight of the i-th
+    int n = 0, slot = 0, again;
+    if (valid) {
+      slot = entry(k0 + ks * lane, n);
+      n = (n - k0 + ks - 1) / ks;
+    }
+    const int nmax = PER == 1 ? n : max(n, __shfl_xor_sync(0xffffffffu, n, 16));
     pdl_wait();
     const float2 none = make_float2(-CUDART_INF_F, 0.f);
     float2 ml = lane < n ? pml[slot] : none;
-    const int flag = t > 0 ? a.flags[s * kvh + g] : 0;
-    V v[U];
-    auto load = [&](int k) {  // entries k .. k + U of the 32 whose slots the lanes hold
+    const int flag = valid && t > 0 ? a.flags[s * kvh + g] : 0;
+    float4 v[U];
+    auto load = [&](int k) {  // entries k .. k + U of the L whose slots the lanes hold
 #pragma unroll
       for (int e = 0; e < U; e++) {
-        const int sl = __shfl_sync(0xffffffffu, slot, (k + e) & 31);
-        if (k + e < n) v[e] = *reinterpret_cast<const V*>(a.part + (size_t)sl * HD + lane * W);
+        const int sl = __shfl_sync(0xffffffffu, slot, (k + e) & (L - 1), L);
+        if (k + e < n) v[e] = *reinterpret_cast<const float4*>(a.part + (size_t)sl * HD + lane * 4);
       }
     };
     load(0);
     float m = ml.x;
 #pragma unroll 1
-    for (int i = 32 + lane; i < n; i += 32) m = fmaxf(m, pml[entry(k0 + ks * i, again)].x);
-    m = warp_max(m);
-    float l = 0.f, acc[W];
+    for (int i = L + lane; i < n; i += L) m = fmaxf(m, pml[entry(k0 + ks * i, again)].x);
 #pragma unroll
-    for (int e = 0; e < W; e++) acc[e] = 0.f;
+    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int base = 0; base < n; base += 32) {
+    for (int base = 0; base < nmax; base += L) {
       if (base > 0) {
-        slot = entry(k0 + ks * (base + lane), again);
+        slot = base + lane < n ? entry(k0 + ks * (base + lane), again) : 0;
         ml = base + lane < n ? pml[slot] : none;
       }
       const float w = ml.x == -CUDART_INF_F ? 0.f : kv_ex2(ml.x - m);
       l += w * ml.y;
 #pragma unroll 1
-      for (int k = base; k < min(n, base + 32); k += U) {
+      for (int k = base; k < min(nmax, base + L); k += U) {
         if (k > 0) load(k);
 #pragma unroll
         for (int e = 0; e < U; e++) {
-          const float wk = __shfl_sync(0xffffffffu, w, (k + e) & 31);
+          const float wk = __shfl_sync(0xffffffffu, w, (k + e) & (L - 1), L);
           if (k + e < n) {
-            const float* f = reinterpret_cast<const float*>(&v[e]);
-#pragma unroll
-            for (int x = 0; x < W; x++) acc[x] += wk * f[x];
+            acc[0] += wk * v[e].x;
+            acc[1] += wk * v[e].y;
+            acc[2] += wk * v[e].z;
+            acc[3] += wk * v[e].w;
           }
         }
       }
     }
-    l = warp_sum(l);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     if constexpr (SPLIT) {
       __syncthreads();  // (the last row's sums have been read)
-      *reinterpret_cast<V*>(&s_acc[warp][lane * W]) = *reinterpret_cast<V*>(acc);
-      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      *reinterpret_cast<float4*>(&s_acc[grp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (lane == 0) s_ml[grp] = make_float2(m, l);
       __syncthreads();
       if (warp != 0) continue;
-      m = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
-      l = 0.f;
+      m = s_ml[0].x;
 #pragma unroll
-      for (int x = 0; x < W; x++) acc[x] = 0.f;
+      for (int e = 1; e < NG; e++) m = fmaxf(m, s_ml[e].x);
+      l = acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
+      for (int e = 0; e < NG; e++) {
         const float w = s_ml[e].x == -CUDART_INF_F ? 0.f : kv_ex2(s_ml[e].x - m);
         l += w * s_ml[e].y;
 #pragma unroll
-        for (int x = 0; x < W; x++) acc[x] += w * s_acc[e][lane * W + x];
+        for (int x = 0; x < 4; x++) acc[x] += w * s_acc[e][lane * 4 + x];
       }
     }
+    if (!valid || (SPLIT && grp != 0)) continue;
     const float inv = 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < W; e++) acc[e] *= inv;
+    for (int e = 0; e < 4; e++) acc[e] *= inv;
     if (flag) {  // infinities and NaN of the block's own V rows that this row sees
 #pragma unroll 1
       for (int tt = 1; tt <= t; tt++) {
         const int pos = q.n + tt;
-        const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * W;
+        const size_t src = ((((size_t)g * a.num_pages + a.tables[q.tab + (pos >> a.shift)]) << a.shift) + (pos & ((1 << a.shift) - 1))) * HD + lane * 4;
 #pragma unroll
-        for (int e = 0; e < W; e += 2) {
+        for (int e = 0; e < 4; e += 2) {
           const uint32_t x = *reinterpret_cast<const uint32_t*>(a.v + src + e);
           const uint32_t nf = kv_nonfinite<BF16>(x);
           const float2 f = kv_unpack<BF16>(x);
@@ -878,17 +885,14 @@ __device__ __forceinline__ void kv_merge(const KvArgs& a, float (*s_acc)[HD], fl
         }
       }
     }
-    uint16_t* out = BT ? a.out + bt_off(orow, head * HD + lane * W, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * W;
-    if constexpr (W == 4)
-      *reinterpret_cast<uint2*>(out) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
-    else
-      *reinterpret_cast<uint32_t*>(out) = kv_pack<BF16>(acc[0], acc[1]);
+    uint16_t* out = BT ? a.out + bt_off(orow, head * HD + lane * 4, H * HD, a.out_bt_n) : a.out + (size_t)orow * a.out_stride + (size_t)head * HD + lane * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(kv_pack<BF16>(acc[0], acc[1]), kv_pack<BF16>(acc[2], acc[3]));
   }
 }
 template <int HD, bool BF16, bool BT>
 __global__ void __launch_bounds__(128, 8) kv_merge_kernel(const KvArgs a) {
-  __shared__ __align__(16) float s_acc[4][HD];
-  __shared__ float2 s_ml[4];
+  __shared__ __align__(16) float s_acc[512 / HD][HD];
+  __shared__ float2 s_ml[512 / HD];
   pdl_trigger();
   if (reinterpret_cast<const KvHdr*>(a.plan)->split_rows)
     kv_merge<HD, BF16, BT, true>(a, s_acc, s_ml);
@@ -1054,9 +1058,9 @@ static void launch_kv_t(const KvWork& w, const KvAttn& a, const KvArgs& k, cudaS
   const size_t smem = KvSmem<HD>::kTotal;
   ensure_smem(kv_attn_kernel<HD, BF16>, smem);
   launch_pdl(kv_attn_kernel<HD, BF16>, dim3(w.g.nctas), dim3(KV_THREADS), smem, s, k, w.qmap, w.qmap_half, *a.kmap, *a.vmap);
-  // a warp per row and head, or a block for each of as many as the plan may split
-  const size_t items = (size_t)a.rows * w.g.heads;
-  const int gm = (int)std::min(std::max((items + 3) / 4, std::min(items, (size_t)w.g.nctas * KV_SPLIT_ITEMS)), (size_t)w.g.nctas * 16);
+  // hd / 4 threads per row and head, or a block for each of as many as the plan may split
+  const size_t items = (size_t)a.rows * w.g.heads, per = 512 / HD;
+  const int gm = (int)std::min(std::max((items + per - 1) / per, std::min(items, (size_t)w.g.nctas * KV_SPLIT_ITEMS)), (size_t)w.g.nctas * 16);
   if constexpr (!BF16) {
     if (a.out_bt) return launch_pdl(kv_merge_kernel<HD, false, true>, dim3(gm), dim3(128), 0, s, k);
   }

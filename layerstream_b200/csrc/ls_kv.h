@@ -44,7 +44,7 @@ void launch_stage(int32_t* table, const KvRange* ranges, int nranges, void* plan
 
 constexpr int KV_TILE = 128;    // query rows of a tile
 constexpr int KV_CHUNK = 128;   // positions of a chunk
-constexpr int KV_SPLIT_ITEMS = 8;  // rows x heads per CTA up to which the merge may take four warps for each
+constexpr int KV_SPLIT_ITEMS = 8;  // rows x heads per SM up to which the merge may take a block for each
 constexpr int KV_LEVELS = 3;    // nodes on a row's path: two shared ranges at most, then its own
 
 struct KvSeg {

@@ -22,9 +22,9 @@ constexpr long long kMinSaved = 256;
 // eight chunks 52.8 against 46.5). A single chunk at 0.55 instead: 64 readers of 32k 68.6 against 65.4 us.
 constexpr double kPairChunk = 1.0, kSingleChunk = 0.62, kPairStart = 1.5, kSingleStart = 0.4;
 
-// A row with more partials than this is merged by four warps instead of one when rows and heads are few
-// (KV_SPLIT_ITEMS). 16 rows of 14 heads, 40 partials: one warp 10.4 us, four 5.6; 288 rows of 16 heads, 10
-// partials: 7.0 and 13.3.
+// A row with more partials than this is merged by a whole block instead of hd / 4 of its threads when rows and
+// heads are few (KV_SPLIT_ITEMS). 16 rows of 14 heads, 40 partials: hd / 4 threads 10.4 us, a block 5.0; 288
+// rows of 16 heads, 10 partials: 7.0 and 13.3.
 constexpr int kSplitRows = 8;
 
 static size_t align16(size_t n) { return (n + 15) / 16 * 16; }
