@@ -184,6 +184,11 @@ def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
 
+def _ints(a):
+    """Arrays as lists: np.array(list, np.int32) refuses what does not fit, a cast of an array would wrap."""
+    return a.tolist() if isinstance(a, np.ndarray) else a
+
+
 def _addr(a: np.ndarray) -> int:
     """The array's address, without _p's cost (4 us); the caller keeps the array."""
     return a.__array_interface__["data"][0]
@@ -615,7 +620,7 @@ class KvCache:
 
     def set_table(self, seq: int, pages, n: int):
         """Sequence seq holds exactly these pages, n positions of them cached."""
-        p = np.ascontiguousarray(pages, np.int32)
+        p = np.array(_ints(pages), np.int32)
         _check(lib().ls_kv_set(self._h, seq, _addr(p), p.size, n))
 
     def fork(self, src: int, dst, n: int | None = None):
@@ -674,8 +679,9 @@ class KvCache:
 def kv_copy_pages(k_ptr: int, v_ptr: int, layers: int, kv_heads: int, hd: int, page: int, num_pages: int, src, dst, rows=None,
                   stream: int = 0):
     """Rows [0, rows[i]) (None: whole pages) of page src[i] to page dst[i], in every layer and kv head of both pools."""
+    lists = [_ints(a) for a in ((src, dst) if rows is None else (src, dst, rows))]
     try:
-        lists = np.array((src, dst) if rows is None else (src, dst, rows), np.int32)  # (one array: small calls are host-bound)
+        lists = np.array(lists, np.int32)  # (one array: small calls are host-bound)
     except ValueError:
         lists = None
     if lists is None or lists.ndim != 2:

@@ -262,3 +262,14 @@ def test_copy_pages_refuses_before_it_touches_the_gpu():
     refuses(call, list(range(16)) + [0], list(range(17)), match="more copies|outside")
     with pytest.raises(ValueError):
         call([0, 1], [2])
+
+
+def test_page_ids_that_do_not_fit_32_bits_are_refused():
+    kv = cache()
+    for ids in ([2**32], np.array([2**32]), np.array([2**31], np.uint64)):
+        with pytest.raises(OverflowError):
+            kv.set_table(0, ids, 0)
+        with pytest.raises(OverflowError):
+            ls.kv_copy_pages(1 << 20, 1 << 20, 1, 1, 64, 16, 8, ids, [0])
+    with pytest.raises(ValueError, match="same length"):
+        ls.kv_copy_pages(1 << 20, 1 << 20, 1, 1, 64, 16, 8, [1, 2], [0])
