@@ -938,6 +938,8 @@ struct KvCopyList {
 template <int N>
 __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ KvCopyList<N> list, int n, uint4* __restrict__ k,
                                                       uint4* __restrict__ v, int blocks, int num_pages, int page16, int row16, int pieces) {
+  pdl_trigger();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const long long warps = (long long)gridDim.x * 8;
   const long long tasks = (long long)n * blocks * 2 * pieces;
@@ -988,9 +990,8 @@ static void launch_copies_t(void* k, void* v, int blocks, int hd, int page, int 
   const int pieces = (rows * row16 + 255) / 256;
   const long long tasks = (long long)runs * blocks * 2 * pieces;
   const int grid = (int)std::min<long long>((tasks + 7) / 8, (long long)num_sms * 8);
-  kv_copy_kernel<N><<<grid, 256, 0, s>>>(list, runs, reinterpret_cast<uint4*>(k), reinterpret_cast<uint4*>(v), blocks, num_pages, page * row16,
-                                         row16, pieces);
-  LS_CUDA(cudaGetLastError());
+  launch_pdl(kv_copy_kernel<N>, dim3(grid), dim3(256), 0, s, list, runs, reinterpret_cast<uint4*>(k), reinterpret_cast<uint4*>(v), blocks,
+             num_pages, page * row16, row16, pieces);
 }
 
 void launch_page_copies(void* k, void* v, int layers, int kv_heads, int hd, int page, int num_pages, const PageCopy* c, size_t n,
@@ -1002,23 +1003,30 @@ void launch_page_copies(void* k, void* v, int layers, int kv_heads, int hd, int 
 }
 
 // The staged parts of a step (host memory that the device reads): block i < n, a run of page-table entries; the
-// others, the plan.
+// others, the plan. What a thread moves first crosses the bus while the kernels before still run.
 __global__ void __launch_bounds__(256) kv_stage_kernel(int32_t* __restrict__ table, const KvRange* __restrict__ ranges, int n,
                                                        uint4* __restrict__ plan, const uint4* __restrict__ staged, int plan16) {
+  pdl_trigger();
   if (blockIdx.x < n) {
     const KvRange r = ranges[blockIdx.x];
     const int32_t* vals = reinterpret_cast<const int32_t*>(ranges + n) + r.from;
-    for (int i = threadIdx.x; i < r.n; i += 256) table[r.at + i] = vals[i];
+    int i = threadIdx.x;
+    int32_t v = i < r.n ? vals[i] : 0;
+    pdl_wait();
+    for (; i < r.n; i += 256, v = i < r.n ? vals[i] : 0) table[r.at + i] = v;
   } else {
-    for (int i = (blockIdx.x - n) * 256 + threadIdx.x; i < plan16; i += (gridDim.x - n) * 256) plan[i] = staged[i];
+    const int step = (gridDim.x - n) * 256;
+    int i = (blockIdx.x - n) * 256 + threadIdx.x;
+    uint4 v = staged[min(i, plan16 - 1)];
+    pdl_wait();
+    for (; i < plan16; i += step, v = staged[min(i, plan16 - 1)]) plan[i] = v;
   }
 }
 
 void launch_stage(int32_t* table, const KvRange* ranges, int nranges, void* plan, const void* staged, size_t plan_bytes, cudaStream_t s) {
   const int plan16 = (int)(plan_bytes / 16);
-  kv_stage_kernel<<<nranges + std::min(64, (plan16 + 255) / 256), 256, 0, s>>>(table, ranges, nranges, static_cast<uint4*>(plan),
-                                                                              static_cast<const uint4*>(staged), plan16);
-  LS_CUDA(cudaGetLastError());
+  launch_pdl(kv_stage_kernel, dim3(nranges + std::min(64, (plan16 + 255) / 256)), dim3(256), 0, s, table, ranges, nranges,
+             static_cast<uint4*>(plan), static_cast<const uint4*>(staged), plan16);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
