@@ -23,8 +23,8 @@
 // grown by more than 2^8 over the one its exponents are taken against.
 //
 // Bound, per two tiles and 128 positions: the special-function units need 2048 clocks for the exponentials
-// (1536 with a quarter of them on the FMA units), the tensor cores 1024 at hd 64 and 2048 at hd 128, HBM
-// 1700 for K and V at hd 128; the kernel takes about 3400. The rest is the latency of a row's chain through
+// (1536 with a quarter of them on the FMA units), the tensor cores 1024 at hd 64 and 2048 at hd 128, an
+// SM's share of HBM 1450 and 2900 for K and V that nobody else reads; the kernel takes about 3400. The rest is the latency of a row's chain through
 // one step (scores out of tensor memory, maximum, exponentials, P into tensor memory, P V, next S). More
 // warps did not hide it: four softmax warpgroups, two for each tile, took 99 us for many pair tiles at hd
 // 128 when they shared a step's columns and 100 when they took the steps in turn, against 90 with two.
