@@ -24,14 +24,15 @@
 //
 // Bound, per two tiles and 128 positions: the special-function units need 2048 clocks for the exponentials
 // (1536 with a quarter of them on the FMA units), the tensor cores 1024 at hd 64 and 2048 at hd 128, an
-// SM's share of HBM 1450 and 2900 for K and V that nobody else reads; the kernel takes about 3400. The rest is the latency of a row's chain through
-// one step (scores out of tensor memory, maximum, exponentials, P into tensor memory, P V, next S). More
-// warps did not hide it: four softmax warpgroups, two for each tile, took 99 us for many pair tiles at hd
-// 128 when they shared a step's columns and 100 when they took the steps in turn, against 90 with two.
+// SM's share of HBM 1450 and 2900 for K and V that nobody else reads; the kernel takes about 3400. The
+// rest is the latency of a row's chain through one step (scores out of tensor memory, maximum,
+// exponentials, P into tensor memory, P V, next S). More warps did not hide it: four softmax warpgroups,
+// two for each tile, took 99 us for many pair tiles at hd 128 when they shared a step's columns and 100
+// when they took the steps in turn, against 90 with two.
 //
 // Rounding: q (after rotation) and P enter the tensor core in the cache's 16-bit type, the type that
 // its operands K and V have; scores, maxima, sums, O and the partials stay f32; the output is rounded
-// once. Infinities and NaN in V rows that only some of a tile's rows may see (the block's own rows)
+// once. (P in a high and a low part takes 8 to 20 % more time.) Infinities and NaN in V rows that only some of a tile's rows may see (the block's own rows)
 // are replaced by zeros for the MMA, since 0 x inf would reach the rows that do not see them, and the
 // merge adds them back to the rows that do.
 #include <cuda_bf16.h>
