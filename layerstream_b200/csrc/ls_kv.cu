@@ -100,14 +100,19 @@ __device__ __forceinline__ float kv_max3_nan(float a, float b, float c) {
 }
 // 2^z on the FMA units, for a share of the exponentials (the special-function units do 16 a clock and SM):
 // z = n + f, n the nearest integer (Cody and Waite's reduction; it sits in the low bits of z + 1.5 * 2^23),
-// 2^f by the quartic with the least largest relative error on [-1/2, 1/2] (Remez exchange, 2.6e-6), n added
-// to the exponent. z is clamped at -126, so the result is at least 2^-126 (ends as zero or next to it
-// in P); z up to 8 occurs. A NaN does not come through: the row's maximum carries it.
+// 2^f by the quartic with the least largest relative error on [-1/2, 1/2] (Remez exchange, 2.7e-6), n added
+// to the exponent; z up to 8 occurs. A NaN does not come through: the row's maximum carries it. In f16 z is clamped
+// at -126: 2^-126 rounds to zero in P. In bf16 it would be a weight, on positions that the row does not see (z =
+// -inf) too; there z is clamped at -127, where the quartic is just below 1, so that taking 127 from its exponent
+// leaves a negative integer, which becomes zero (every z <= -127 then gives zero, and what lies between -127 and
+// -126 is off by at most 2^-127; ex2.approx.ftz flushes it).
 // Many pair tiles at hd 128 and 64: no share 93.7 and 79.8 us, a quarter 89.7 and 77.3, 3/8 90.4 and
 // 77.4, half 94.1 and 80.9.
+template <bool BF16>
 __device__ __forceinline__ float2 kv_ex2_fma(uint64_t z) {
+  constexpr float LOW = BF16 ? -127.f : -126.f;
   const float2 zf = kv_un2(z);
-  z = kv_f2(fmaxf(zf.x, -126.f), fmaxf(zf.y, -126.f));
+  z = kv_f2(fmaxf(zf.x, LOW), fmaxf(zf.y, LOW));
   const uint64_t r = kv_add2(z, kv_f2(12582912.f, 12582912.f));
   const uint64_t f = kv_fma2(kv_add2(r, kv_f2(-12582912.f, -12582912.f)), kv_f2(-1.f, -1.f), z);
   uint64_t p = kv_f2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
@@ -116,8 +121,9 @@ __device__ __forceinline__ float2 kv_ex2_fma(uint64_t z) {
   p = kv_fma2(p, f, kv_f2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
   p = kv_fma2(p, f, kv_f2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
   const float2 pf = kv_un2(p), rf = kv_un2(r);
-  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23)),
-                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23)));
+  int x = __float_as_int(pf.x) + (__float_as_int(rf.x) << 23), y = __float_as_int(pf.y) + (__float_as_int(rf.y) << 23);
+  if constexpr (BF16) x = max(x, 0), y = max(y, 0);
+  return make_float2(__int_as_float(x), __int_as_float(y));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
@@ -705,7 +711,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
               const uint64_t z = kv_fma2(kv_f2(x[q * 32 + 2 * e], x[q * 32 + 2 * e + 1]), cs2, mb2);
               float2 w;
               if ((e & 3) == 2) {
-                w = kv_ex2_fma(z);
+                w = kv_ex2_fma<BF16>(z);
               } else {
                 w = kv_un2(z);
                 w.x = kv_ex2(w.x);

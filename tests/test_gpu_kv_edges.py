@@ -1,0 +1,47 @@
+"""Attention over shared pages at its edges (needs a B200): what a row must not see, plans of more levels and segments, and
+calls in orders that the other tests do not make. Tolerances are those of test_gpu_kv.py."""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv import Setup, run_layer
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("hd,dtype,n,M", [(64, "f16", 100, 6), (128, "bf16", 125, 9), (64, "bf16", 0, 40), (128, "bf16", 10, 130)])
+def test_the_largest_values_in_new_rows_reach_only_the_rows_that_see_them(hd, dtype, n, M):
+    s = Setup(4, 2, hd, dtype, 16, 2, M, n + M, seed=3)
+    s.fill_fast(0, list(range(-(-n // 16))), n)
+    s.fill_fast(1, list(range(-(-n // 16), 2 * -(-n // 16))), n)
+    s.kv.begin([M, M], M)
+    qkv = s.randn(2 * M, s.W)
+    ref = run_layer(s, 0, [M, M], qkv).view(2, M, 4, hd)
+    big = torch.finfo(s.dt).max
+    v = (4 + 2) * hd
+    for t0 in (M // 2, M - 1):  # every row from t0 on, in some columns of both kv heads
+        bad = qkv.clone()
+        bad[t0:M, v + 3] = big
+        bad[t0:M, v + hd + 5] = -big
+        got = run_layer(s, 0, [M, M], bad, check=False).view(2, M, 4, hd)
+        assert torch.equal(got[1], ref[1])
+        assert torch.equal(got[0, :t0], ref[0, :t0]), t0
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, "f16"), (64, "bf16"), (128, "bf16")])
+def test_a_weight_of_zero_takes_nothing_from_the_largest_value(hd, dtype):
+    # eight neighbouring keys whose scores are 2 hd below zero: their weights are zero in 32 bits
+    s = Setup(4, 2, hd, dtype, 16, 3, 2, 330, seed=9)
+    s.fill_fast(0, list(range(20)), 300)
+    s.k[0, :, 3, 4:12] = -2 * math.sqrt(hd)
+    s.kv.fork(0, [1, 2])
+    s.kv.begin([2, 2, 2], 2)
+    qkv = s.randn(6, s.W)
+    qkv[:, : 4 * hd] = 1
+    s.v[0, :, 3, 4:12] = 0
+    ref = run_layer(s, 0, [2, 2, 2], qkv, rope=False, check=False)
+    s.v[0, :, 3, 4:12] = torch.finfo(s.dt).max
+    got = run_layer(s, 0, [2, 2, 2], qkv, rope=False, check=False)
+    assert torch.isfinite(ref).all() and torch.equal(got, ref)
