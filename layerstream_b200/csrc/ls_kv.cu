@@ -1056,7 +1056,7 @@ void kv_encode_map(CUtensorMap* m, const void* base, uint64_t rows, int hd, int 
   if (r != CUDA_SUCCESS) LS_THROW(LS_ERR_CUDA, "cuTensorMapEncodeTiled (K/V cache) failed: " + std::to_string((int)r));
 }
 
-void KvWork::open(const KvGeom& geom, bool is_bf16, int* err_word) {
+void KvWork::open(const KvGeom& geom, bool is_bf16, int* err_word, cudaStream_t s) {
   g = geom;
   bf16 = is_bf16;
   err = err_word;
@@ -1069,9 +1069,10 @@ void KvWork::open(const KvGeom& geom, bool is_bf16, int* err_word) {
   q = p + bp;
   part = reinterpret_cast<float*>(p + bp + bq);
   flags = reinterpret_cast<int*>(p + bp + bq + bo);
-  // the query operand's rows past the block's are read into tiles (and never used): finite from the start
-  LS_CUDA(cudaMemset(q, 0, bq));
-  LS_CUDA(cudaMemset(flags, 0, bf));
+  // the query operand's rows past the block's are read into tiles (and never used): finite from the start. In the
+  // order of the stream that uses them first: cudaMemset's is the legacy stream, which a non-blocking one passes.
+  LS_CUDA(cudaMemsetAsync(q, 0, bq, s));
+  LS_CUDA(cudaMemsetAsync(flags, 0, bf, s));
   kv_encode_map(&qmap, q, qrows, g.hd, KV_TILE, bf16);
   kv_encode_map(&qmap_half, q, qrows, g.hd, KV_TILE / 2, bf16);
 }

@@ -162,7 +162,7 @@ struct KvWork {
   int* err = nullptr;          // device-visible error word (1: a bounded wait gave up)
   CUtensorMap qmap{}, qmap_half{};  // boxes of a tile's rows, of half a tile's
   void* mem = nullptr;         // the allocation behind plan, q, part and flags
-  void open(const KvGeom& geom, bool is_bf16, int* err_word);  // on the current device
+  void open(const KvGeom& geom, bool is_bf16, int* err_word, cudaStream_t s);  // on the current device; cleared in s's order
   void close();
 };
 

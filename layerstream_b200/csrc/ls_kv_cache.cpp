@@ -197,7 +197,7 @@ struct LsKv {
     const size_t entries = (size_t)g.nseq * g.max_pages;
     LS_CUDA(cudaMalloc(&d_table, entries * 4));
     LS_CUDA(cudaMemset(d_table, 0, entries * 4));
-    work.open(g, bf16, d_err);
+    work.open(g, bf16, d_err, nullptr);  // (waited for below: steps may run on any stream)
     maps.resize(2 * layers);
     for (size_t l = 0; l < layers; l++)
       for (int i = 0; i < 2; i++)

@@ -2152,7 +2152,7 @@ struct LsBatch {
         for (int i = 0; i < 2; i++)
           kv_encode_map(&kv_maps[2 * l + i], (i ? vc : kc) + l * kv_layer, (uint64_t)dm.kv_heads * pool.num_pages << pool.shift, hd,
                         kv_box_rows(pool.page()), false);
-      kvw.open(g, false, d_err);
+      kvw.open(g, false, d_err, stream);
     }
     std::vector<KvSeqIn> in(ns);
     for (size_t i = 0; i < ns; i++) {
