@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   const KvProg pr = reinterpret_cast<const KvProg*>(a.plan + h.off_prog)[blockIdx.x];
   const KvSeg* const segs = reinterpret_cast<const KvSeg*>(a.plan + h.off_seg);
   pdl_trigger();
-  if (pr.nseg[0] + pr.nseg[1] == 0) return;
+  if (pr.nseg[0] + pr.nseg[1] == 0) return pdl_wait();  // (when this grid has ended, the one before it has: in a step without rows too)
 
   constexpr int SEG16 = sizeof(KvSeg) / 16;
   static_assert(sizeof(KvSeg) % 16 == 0, "segments are copied in 16-byte pieces");

@@ -45,3 +45,29 @@ def test_a_weight_of_zero_takes_nothing_from_the_largest_value(hd, dtype):
     s.v[0, :, 3, 4:12] = torch.finfo(s.dt).max
     got = run_layer(s, 0, [2, 2, 2], qkv, rope=False, check=False)
     assert torch.isfinite(ref).all() and torch.equal(got, ref)
+
+
+def test_steps_without_rows_between_steps_with_rows():
+    # queued without a wait: the rows that an empty step's kernels find are never those of the step behind it
+    pools = []
+    for empty in (False, True):
+        s = Setup(8, 2, 64, "f16", 16, 4, 3, 700, layers=2, seed=13)
+        s.fill_fast(0, list(range(20)), 310)
+        s.kv.fork(0, [1, 2, 3])
+        qkv, other, out = s.randn(100, 12, s.W), s.randn(12, s.W), torch.zeros(12, 8 * 64, device="cuda", dtype=s.dt)
+        torch.cuda.synchronize()
+        outs = []
+        for i in range(100):
+            if empty:
+                s.kv.begin([0, 0, 0, 0], 3)
+                for layer in (0, 1):
+                    s.kv.attention(layer, other.data_ptr(), out.data_ptr(), s.rope.data_ptr())
+            s.kv.begin([3, 2, 0, 1], 3)
+            for layer in (0, 1):
+                s.kv.attention(layer, qkv[i].data_ptr(), out.data_ptr(), s.rope.data_ptr())
+            outs.append(out.clone())
+            s.kv.end([1, 2, 0, 1])
+        torch.cuda.synchronize()
+        pools.append([torch.stack(outs), s.k.view(torch.int16), s.v.view(torch.int16)])
+    for a, b in zip(*pools):
+        assert torch.equal(a, b)
