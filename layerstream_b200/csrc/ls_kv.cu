@@ -354,7 +354,6 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   const KvHdr& h = *reinterpret_cast<const KvHdr*>(a.plan);
   const KvProg pr = reinterpret_cast<const KvProg*>(a.plan + h.off_prog)[blockIdx.x];
   const KvSeg* const segs = reinterpret_cast<const KvSeg*>(a.plan + h.off_seg);
-  pdl_trigger();
   if (pr.nseg[0] + pr.nseg[1] == 0) return pdl_wait();  // (when this grid has ended, the one before it has: in a step without rows too)
 
   constexpr int SEG16 = sizeof(KvSeg) / 16;
@@ -389,6 +388,9 @@ __global__ void __launch_bounds__(KV_THREADS, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  // Only now: a kernel two launches on (the next product) takes tensor memory before it waits for this one. Were it
+  // let onto the SM first, the allocation here could wait for it, and it for this kernel.
+  pdl_trigger();
   const uint32_t tmem = s_tmem;
   // Ring use of lane t's chunk: pair chunk i is in stage i % NS of K and of V; chunk j of a lane's own
   // phase in stage (2 j + t) % NS, so that each lane's own stages advance with that lane alone. Its
