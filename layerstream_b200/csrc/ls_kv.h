@@ -112,7 +112,7 @@ class KvPlanner {
   KvGeom g;
   std::vector<uint8_t> bytes;  // the packed plan (KvHdr first)
   // version: changes whenever a page table changed other than by growing at its end (the sharing
-  // tree of the last plan is kept while version and the set of sequences with rows stay the same).
+  // tree of the last plan is kept while version and every sequence's class, by its rows, stay the same).
   void build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version);
   // Throws unless the plan covers every row's positions exactly once and stays inside its bounds.
   void check(const std::vector<KvSeqIn>& seqs) const;
@@ -133,7 +133,8 @@ class KvPlanner {
   };
   std::vector<int> order_;   // sequences with rows, in plan order
   std::vector<Node> shared_; // shared ranges
-  std::vector<uint8_t> active_;
+  enum Class : uint8_t { IDLE, GROUPED, ALONE };  // no rows; planned with those that share its pages; by itself
+  std::vector<Class> class_;
   uint64_t version_ = ~0ull;
   size_t shared_pos_ = 0;
   std::vector<Node> nodes_;
@@ -147,6 +148,7 @@ class KvPlanner {
   std::vector<KvSeg> segs_, lane_[2];
   std::vector<KvProg> progs_;
   std::vector<KvUnit> units_;
+  Class class_of(int cnt) const;
   void tree(const std::vector<KvSeqIn>& seqs);
 };
 

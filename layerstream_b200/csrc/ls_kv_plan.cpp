@@ -43,12 +43,7 @@ void KvPlanner::tree(const std::vector<KvSeqIn>& seqs) {
   shared_.clear();
   std::vector<int> act, alone;
   for (size_t i = 0; i < seqs.size(); i++)
-    if (seqs[i].cnt > 0) {
-      // rows that fill tiles of their own read the prefix once per pair of tiles either way: as one range with
-      // their own positions they leave one partial less
-      const int rows = seqs[i].cnt * g.G(), pairs = (rows + 2 * KV_TILE - 1) / (2 * KV_TILE);
-      (rows * 5 >= pairs * 2 * KV_TILE * 4 ? alone : act).push_back((int)i);
-    }
+    if (class_[i] != IDLE) (class_[i] == ALONE ? alone : act).push_back((int)i);
   auto full = [&](int i) { return seqs[i].n >> g.shift; };
   // runs of `ids` that agree on the page at depth d, in order of first appearance; sequences without a
   // full page there come last, one by one
@@ -101,12 +96,20 @@ void KvPlanner::tree(const std::vector<KvSeqIn>& seqs) {
   order_.insert(order_.end(), alone.begin(), alone.end());
 }
 
+KvPlanner::Class KvPlanner::class_of(int cnt) const {
+  if (cnt == 0) return IDLE;
+  // rows that fill tiles of their own read the prefix once per pair of tiles either way: as one range with
+  // their own positions they leave one partial less
+  const int rows = cnt * g.G(), pairs = (rows + 2 * KV_TILE - 1) / (2 * KV_TILE);
+  return rows * 5 >= pairs * 2 * KV_TILE * 4 ? ALONE : GROUPED;
+}
+
 void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version) {
-  std::vector<uint8_t> act(seqs.size());
-  for (size_t i = 0; i < seqs.size(); i++) act[i] = seqs[i].cnt > 0;
-  if (version != version_ || act != active_) {
+  std::vector<Class> now(seqs.size());
+  for (size_t i = 0; i < seqs.size(); i++) now[i] = class_of(seqs[i].cnt);
+  if (version != version_ || now != class_) {
+    class_ = now;
     tree(seqs);
-    active_ = act;
     version_ = version;
   }
   const int G = g.G(), kvh = g.kv_heads;

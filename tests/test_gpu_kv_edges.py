@@ -71,3 +71,17 @@ def test_steps_without_rows_between_steps_with_rows():
         pools.append([torch.stack(outs), s.k.view(torch.int16), s.v.view(torch.int16)])
     for a, b in zip(*pools):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("heads,hd,dtype", [(14, 64, "f16"), (16, 128, "bf16")])
+def test_prompts_continued_under_a_shared_prompt_then_single_rows(heads, hd, dtype):
+    # blocks that are planned by themselves, then steps that read the prefix once, and back
+    s = Setup(heads, 2, hd, dtype, 64, 4, 128, 1400, seed=17)
+    s.fill_fast(0, list(range(16)), 1000)
+    s.kv.fork(0, [1, 2, 3])
+    for counts, shared in (([128] * 4, 0), ([1] * 4, 960), ([2, 1, 2, 1], 960), ([128, 1, 128, 1], 960), ([128] * 4, 0), ([1] * 4, 960)):
+        s.kv.begin(counts, 128)
+        s.kv.self_check()
+        assert s.kv.info.shared_positions == shared, counts
+        run_layer(s, 0, counts)
+        s.kv.end()

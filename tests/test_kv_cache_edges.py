@@ -1,0 +1,38 @@
+"""Steps of ls.KvCache in orders and with arguments that the other tests do not make (no GPU: device=-1)."""
+
+import numpy as np
+import pytest
+
+import layerstream_b200 as ls
+from test_kv_cache import cache, refuses
+
+
+def prompts(n, seqs=8, M=128, page=64):
+    """Sequences forked under the same n positions."""
+    kv = cache(seqs=seqs, page=page, num_pages=n // page + 1 + seqs * 8, max_ctx=n + 512, max_rows=seqs * M, heads=14, kv_heads=2)
+    kv.set_table(0, range(-(-n // page)), n)
+    kv.fork(0, range(1, seqs))
+    return kv
+
+
+@pytest.mark.parametrize("n", [4096, 4100])
+@pytest.mark.parametrize("rows", [[128, 1, 1], [1, 128, 1], [1, 32, 5, 128, 128, 2], [33, 40, 33]])
+def test_what_a_step_shares_depends_on_its_own_rows_alone(n, rows):
+    # (32, 33 or 128 rows of 7 heads fill four fifths of their pairs of tiles and are planned alone, the others are not)
+    kv = prompts(n)
+    for r in rows:
+        kv.begin([r] * 8, 128)
+        kv.self_check()
+        fresh = prompts(n)
+        fresh.begin([r] * 8, 128)
+        assert kv.info.shared_positions == fresh.info.shared_positions == (0 if r in (32, 33, 128) else 4096), r
+        kv.end()
+
+
+def test_sequences_with_many_rows_beside_sequences_with_few():
+    kv = prompts(4096)
+    for counts in ([128] * 4 + [1] * 4, [1] * 4 + [128] * 4, [1] * 8, [0, 0, 0, 1, 0, 0, 128, 128], [2] * 8):
+        kv.begin(counts, 128)
+        kv.self_check()
+        few = sum(1 for c in counts if 0 < c < 100)
+        assert kv.info.shared_positions == (4096 if few > 1 else 0), counts
