@@ -304,7 +304,7 @@ struct LsKv {
 
   // A step: sequence s is to get cnt[s] rows (0..M) behind its cached positions.
   void begin(const uint32_t* cnt, uint64_t M, cudaStream_t st) {
-    if (M == 0 || M * (uint64_t)g.nseq > (uint64_t)g.max_rows) LS_THROW(LS_ERR_ARG, "seqs x M must be in 1..max_rows");
+    if (M == 0 || M > (uint64_t)g.max_rows / g.nseq) LS_THROW(LS_ERR_ARG, "seqs x M must be in 1..max_rows");
     if (device >= 0) {
       check_err();
       if (capturing(st)) LS_THROW(LS_ERR_ARG, "a step cannot begin while the stream is being captured");

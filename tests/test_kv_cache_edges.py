@@ -36,3 +36,12 @@ def test_sequences_with_many_rows_beside_sequences_with_few():
         kv.self_check()
         few = sum(1 for c in counts if 0 < c < 100)
         assert kv.info.shared_positions == (4096 if few > 1 else 0), counts
+
+
+@pytest.mark.parametrize("M", [2**62, 2**63, 2**63 + 1, 2**64 - 1, 5])
+def test_begin_refuses_more_rows_than_the_workspaces_hold(M):
+    # seqs x M of the large ones is 0, 0, 4 and -4 modulo 2^64
+    kv = cache(seqs=4, max_rows=16)
+    refuses(kv.begin, [1, 1, 1, 1], M, match="max_rows")
+    assert kv.info.pages_used == 0
+    kv.self_check()
