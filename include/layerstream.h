@@ -281,7 +281,8 @@ int ls_batch_tp_peer(const LsBatch *b, int *on);
  * its length: pages are taken (the lowest free ones), shared pages among those that will be written are copied in
  * every layer, and the pass's plan is laid out; ls_kv_attention once per layer; ls_kv_end keeps the
  * first keep[s] of the rows (NULL: all) and returns the pages past them. A step that was begun and not
- * ended is dropped by the next begin, and by any call that changes a table.
+ * ended is dropped by the next begin, and by any call that changes a table. A begin that fails leaves the
+ * tables as they were.
  *
  * Calls on one cache come from one thread at a time, and their GPU work, on whichever streams, must
  * not overlap (the caller orders the streams). ls_kv_begin and ls_kv_compact are refused on a stream
@@ -331,6 +332,10 @@ int ls_kv_end(LsKv *kv, const uint32_t *keep);
 /* LS_ERR_ARG unless the page counts agree with the tables and the begun step's plan covers every row's
  * positions exactly once (for tests; host work alone). */
 int ls_kv_self_check(const LsKv *kv);
+/* Test hook, no reference counterpart; nothing faults on the GPU. code 1: the next ls_kv_begin fails with LS_ERR_CUDA where
+ * its launches would; 2 (with a GPU): the error word reads as if an attention kernel's bounded wait had run out. 0 clears a
+ * pending 1. */
+int ls_kv_inject_error(LsKv *kv, int code);
 /* Copies rows [0, rows[i]) (NULL: whole pages) of page src[i] to page dst[i] in every layer and kv head of both
  * pools, for pools as above of any head size that is a multiple of 8. src, dst, rows: host memory. No page may be
  * written twice, or both read and written. */

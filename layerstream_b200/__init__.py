@@ -135,6 +135,7 @@ _SIGS = {
     "ls_kv_attention": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     "ls_kv_end": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ls_kv_self_check": (C.c_int, [C.c_void_p]),
+    "ls_kv_inject_error": (C.c_int, [C.c_void_p, C.c_int]),
     "ls_kv_copy_pages": (C.c_int, [C.c_void_p, C.c_void_p] + [C.c_uint64] * 5 + [C.c_void_p] * 3 + [C.c_uint64, C.c_void_p]),
     "ls_attention_host": (C.c_int, [C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_uint64, C.c_uint64, C.c_void_p,
                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_double)]),
@@ -654,6 +655,10 @@ class KvCache:
 
     def self_check(self):
         _check(lib().ls_kv_self_check(self._h))
+
+    def inject_error(self, code: int = 1):
+        """Test hook: the next ``begin`` fails at its launches (1), or a kernel has given up waiting (2); no fault on the GPU."""
+        _check(lib().ls_kv_inject_error(self._h, code))
 
     def _per_seq(self, a) -> array:
         try:

@@ -477,6 +477,7 @@ void kv_attention(LsKv* kv, uint64_t layer, const void* qkv, uint64_t qkv_stride
                   cudaStream_t st);
 void kv_end(LsKv* kv, const uint32_t* keep);
 void kv_self_check(const LsKv* kv);
+void kv_inject(LsKv* kv, int code);
 void kv_info(const LsKv* kv, LsKvInfo* out);
 uint64_t kv_len(const LsKv* kv, uint64_t s);
 void kv_tables(const LsKv* kv, int32_t* out);

@@ -97,6 +97,7 @@ struct LsKv {
   int turn = 0;
   int *h_err = nullptr, *d_err = nullptr;  // error word, mapped
   std::vector<PageCopy> copies;
+  bool inject_fail = false;  // test hook: the next step's launches fail
 
   LsKv() = default;
   LsKv(const LsKv&) = delete;
@@ -327,27 +328,54 @@ struct LsKv {
     if (need > nfree) LS_THROW(LS_ERR_ARG, "the K/V page pool is exhausted: " + std::to_string(need) + " pages needed, " + std::to_string(nfree) + " free");
     begun = false;
     copies.clear();
-    for (int s = 0; s < g.nseq; s++) {
-      counts[s] = (int)cnt[s];
-      if (cnt[s] == 0) continue;
-      const int last = pages_of((size_t)len[s] + cnt[s]);
-      for (int i = len[s] >> g.shift; i < last; i++) {
-        if (i >= held[s]) {
-          row(s)[i] = take();
-          held[s] = i + 1;
-          touch(s, i, i + 1);
-        } else if (ref[row(s)[i]] > 1) {
-          const int old = row(s)[i], rows = std::max(0, len[s] - (i << g.shift));
-          row(s)[i] = take();
-          drop(old);
-          if (rows) copies.push_back({old, row(s)[i], rows});
-          touch(s, i, i + 1);
-          version++;
+    struct Entry {
+      int s, i;
+      int32_t before;  // -1: the sequence has grown by this page
+    };
+    std::vector<Entry> entries;  // table entries that the step changes
+    try {
+      for (int s = 0; s < g.nseq; s++) {
+        counts[s] = (int)cnt[s];
+        if (cnt[s] == 0) continue;
+        const int last = pages_of((size_t)len[s] + cnt[s]);
+        for (int i = len[s] >> g.shift; i < last; i++) {
+          if (i >= held[s]) {
+            entries.push_back({s, i, -1});
+            row(s)[i] = take();
+            held[s] = i + 1;
+            touch(s, i, i + 1);
+          } else if (ref[row(s)[i]] > 1) {
+            const int old = row(s)[i], rows = std::max(0, len[s] - (i << g.shift));
+            if (rows) copies.push_back({old, -1, rows});
+            entries.push_back({s, i, old});
+            row(s)[i] = take();
+            drop(old);
+            if (rows) copies.back().dst = row(s)[i];
+            touch(s, i, i + 1);
+            version++;
+          }
         }
       }
+      planner.build(inputs(), (int)M, version);
+      if (inject_fail) LS_THROW(LS_ERR_CUDA, "the step's launches failed (test hook)");
+      if (device >= 0) upload(st);
+    } catch (...) {
+      // the copies may not have been made: the tables are what they were, and go up whole with the next step
+      inject_fail = false;
+      for (size_t e = entries.size(); e-- > 0;) {
+        const Entry& x = entries[e];
+        drop(row(x.s)[x.i]);
+        if (x.before < 0) {
+          held[x.s] = x.i;
+        } else {
+          row(x.s)[x.i] = x.before;
+          ref[x.before]++;
+        }
+      }
+      for (int s = 0; s < g.nseq; s++) touch(s, 0, held[s]);
+      changed();
+      throw;
     }
-    planner.build(inputs(), (int)M, version);
-    if (device >= 0) upload(st);
     begun = true;
   }
 
@@ -435,6 +463,12 @@ struct LsKv {
     begun = false;
   }
 
+  void inject(int code) {
+    if (code < 0 || code > 2 || (code == 2 && device < 0)) LS_THROW(LS_ERR_ARG, "the injected error must be 0, 1 or (with a GPU) 2");
+    inject_fail = code == 1;
+    if (code == 2) *reinterpret_cast<volatile int*>(h_err) = 1;
+  }
+
   // Throws unless the pages' counts, the free count and the plan agree with the tables.
   void self_check() const {
     std::vector<int32_t> count(g.num_pages, 0);
@@ -488,6 +522,7 @@ void kv_attention(LsKv* kv, uint64_t layer, const void* qkv, uint64_t qkv_stride
 }
 void kv_end(LsKv* kv, const uint32_t* keep) { kv->end(keep); }
 void kv_self_check(const LsKv* kv) { kv->self_check(); }
+void kv_inject(LsKv* kv, int code) { kv->inject(code); }
 void kv_info(const LsKv* kv, LsKvInfo* o) {
   o->seqs = kv->g.nseq;
   o->max_pages = kv->g.max_pages;

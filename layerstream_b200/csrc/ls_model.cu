@@ -3104,6 +3104,13 @@ int ls_kv_self_check(const LsKv* kv) {
   });
 }
 
+int ls_kv_inject_error(LsKv* kv, int code) {
+  return guard([&] {
+    NEED(kv);
+    kv_inject(kv, code);
+  });
+}
+
 int ls_kv_copy_pages(void* k_pool, void* v_pool, uint64_t layers, uint64_t kv_heads, uint64_t hd, uint64_t page, uint64_t num_pages,
                      const int32_t* src, const int32_t* dst, const int32_t* rows, uint64_t n, void* stream) {
   return guard([&] { kv_copy_pages(k_pool, v_pool, layers, kv_heads, hd, page, num_pages, src, dst, rows, n, reinterpret_cast<cudaStream_t>(stream)); });

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import layerstream_b200 as ls
 from test_gpu_kv import Setup, run_layer
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,20 @@ def test_prompts_continued_under_a_shared_prompt_then_single_rows(heads, hd, dty
         assert s.kv.info.shared_positions == shared, counts
         run_layer(s, 0, counts)
         s.kv.end()
+
+
+def test_a_begin_that_failed_is_made_again_with_its_copies():
+    s = Setup(4, 2, 64, "f16", 16, 4, 3, 400, layers=2, seed=19)
+    s.fill_fast(0, list(range(20)), 309)  # the last page is shared in part: three of the four holders copy it
+    s.kv.fork(0, [1, 2, 3])
+    before = s.kv.tables()
+    for _ in range(2):
+        s.kv.inject_error()
+        with pytest.raises(ls.LayerstreamError, match="test hook") as e:
+            s.kv.begin([3, 1, 2, 3], 3)
+        assert e.value.code == -3 and (s.kv.tables() == before).all()
+    s.kv.begin([3, 1, 2, 3], 3)
+    s.kv.self_check()
+    for layer in (0, 1):
+        run_layer(s, layer, [3, 1, 2, 3])
+    s.kv.end()

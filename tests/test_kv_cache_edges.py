@@ -45,3 +45,50 @@ def test_begin_refuses_more_rows_than_the_workspaces_hold(M):
     refuses(kv.begin, [1, 1, 1, 1], M, match="max_rows")
     assert kv.info.pages_used == 0
     kv.self_check()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_a_begin_that_fails_changes_nothing(seed):
+    # forks, rollbacks and dropped steps; now and then a begin fails at its launches, and is then made again: the
+    # tables are always those of a cache where none failed
+    rng = np.random.default_rng(seed)
+    a, b = (cache(seqs=5, page=8, num_pages=60, max_ctx=96, max_rows=60) for _ in range(2))
+    both = (a, b)
+    for step in range(50):
+        what = rng.integers(0, 5)
+        if what == 0:
+            src = int(rng.integers(5))
+            dst = [int(d) for d in rng.permutation(5)[:2] if d != src]
+            n = int(rng.integers(0, a.length(src) + 1))
+            for kv in both:
+                kv.fork(src, dst, n)
+        elif what == 1:
+            s = int(rng.integers(5))
+            n = int(rng.integers(0, a.length(s) + 1))
+            for kv in both:
+                kv.truncate(s, n)
+        else:
+            counts = [int(min(rng.integers(0, 13), 96 - a.length(s))) for s in range(5)]
+            before, info = a.tables(), a.info
+            a.inject_error()
+            refuses(a.begin, counts, 12, match="test hook", code=-3)
+            a.self_check()
+            assert np.array_equal(a.tables(), before)
+            assert (a.info.pages_used, a.info.pages_shared) == (info.pages_used, info.pages_shared)
+            refuses(a.end, match="no step")
+            for kv in both:
+                kv.begin(counts, 12)
+            a.self_check()
+            assert a.info.shared_positions == b.info.shared_positions
+            assert np.array_equal(a.tables(), b.tables())
+            if what < 4:
+                keep = [int(rng.integers(0, c + 1)) for c in counts]
+                for kv in both:
+                    kv.end(keep)
+        a.self_check()
+        assert np.array_equal(a.tables(), b.tables()), step
+    a.inject_error()
+    a.inject_error(0)
+    a.begin([0] * 5, 1)
+    for code in (-1, 2, 3):
+        refuses(a.inject_error, code)
