@@ -252,8 +252,9 @@ int ls_model_inject_stall(LsModel *m, int barrier);
  * failing Source, tests/pipeline.rs:170-198): the batch's next pass reports error code 4 from the
  * device as a failed kernel would, without any fault on the GPU. On a tensor-parallel batch the
  * error word is reduced over the ranks, so injecting on one rank makes every rank's pass fail with
- * LS_ERR_DEVICE; a batch whose pass failed releases its communicator with ncclCommAbort. code 0
- * clears a pending injection. */
+ * LS_ERR_DEVICE; a batch whose pass failed releases its communicator with ncclCommAbort. code 6: the
+ * next pass that copies shared pages fails there with LS_ERR_CUDA, before anything else of it runs (a pass
+ * without copies runs and clears it). code 0 clears a pending injection. */
 int ls_batch_inject_error(LsBatch *b, int code);
 /* on: 0 off, 1 an event pair around every launch class of each pass; also clears the counters */
 int ls_batch_profile_enable(LsBatch *b, int on);

@@ -126,18 +126,32 @@ struct PagePool {
     if (need) upload(d, 0, need, st);
   }
   // Before sequence s (n positions) writes positions [n, end): of its pages there, those that others
-  // hold too are replaced by new ones, their rows in use to be copied. (The pool never runs out: it has
-  // a page for every table entry, and two entries that share one leave one over.)
-  void own_rows(int s, size_t n, size_t end, std::vector<PageCopy>& copies, cudaStream_t st) {
+  // hold too get a successor, with their rows in use to be copied; the tables change once the copies are under way
+  // (rename; give_back when they could not be made). (The pool never runs out: it has a page for every table entry,
+  // and two entries that share one leave one over.)
+  struct Move {
+    int s, i;
+    int32_t page;
+  };
+  void own_rows(int s, size_t n, size_t end, std::vector<PageCopy>& copies, std::vector<Move>& moves) {
     const int last = std::min(held[s], (int)((end + page() - 1) >> shift));
     for (int i = (int)(n >> shift); nshared && i < last; i++) {
       const int32_t old = row(s)[i];
       if (ref[old] == 1) continue;
-      row(s)[i] = take();
+      moves.push_back({s, i, take()});
       drop(old);
-      if (n > (size_t)i << shift) copies.push_back({old, row(s)[i], (int32_t)(n - ((size_t)i << shift))});
-      version++;
-      upload(s, i, i + 1, st);
+      if (n > (size_t)i << shift) copies.push_back({old, moves.back().page, (int32_t)(n - ((size_t)i << shift))});
+    }
+  }
+  void rename(const std::vector<Move>& moves, cudaStream_t st) {
+    for (const Move& m : moves) row(m.s)[m.i] = m.page;
+    version += moves.size();
+    for (const Move& m : moves) upload(m.s, m.i, m.i + 1, st);
+  }
+  void give_back(const std::vector<Move>& moves) {
+    for (size_t k = moves.size(); k-- > 0;) {
+      hold(row(moves[k].s)[moves[k].i]);
+      drop(moves[k].page);
     }
   }
   int used() const { return num_pages - (int)free_list.size(); }
@@ -1600,9 +1614,11 @@ struct LsBatch {
   std::vector<CUtensorMap> kv_maps;            // [layers] K, V
   uint8_t* h_plan = nullptr;
   std::vector<PageCopy> copies;
+  std::vector<PagePool::Move> moves;
   uint32_t *h_tok = nullptr, *h_m = nullptr, *h_next = nullptr;
   int *h_pos0 = nullptr, *h_err = nullptr;
-  int inject_err = 0;      // test hook: the next pass reports this error code (a host-made fault)
+  int inject_err = 0;      // test hook: the next pass reports this error code (a host-made fault), or fails at its page copies
+  static constexpr int kInjectCopies = 6;
   bool tp_failed = false;  // a tensor-parallel pass reported an error
   std::vector<uint64_t> pos;
   uint64_t passes = 0, h2d_bytes = 0, d2h_bytes = 0;
@@ -2186,14 +2202,22 @@ struct LsBatch {
     }
     for (size_t i = 0; i < T; i++)
       if (tokens[i] >= c.vocab) LS_THROW(LS_ERR_ARG, "token id " + std::to_string(tokens[i]) + " is outside the vocabulary");
+    // pages for the new rows, none of them anyone else's
     copies.clear();
-    for (size_t i = 0; i < ns; i++) {  // pages for the new rows, none of them anyone else's
-      pool.own_rows((int)(s0 + i), pos[s0 + i], pos[s0 + i] + M, copies, stream);
-      pool.ensure((int)(s0 + i), pos[s0 + i] + M, stream);
+    moves.clear();
+    for (size_t i = 0; i < ns; i++) pool.own_rows((int)(s0 + i), pos[s0 + i], pos[s0 + i] + M, copies, moves);
+    try {
+      if (!moves.empty() && inject_err == kInjectCopies) LS_THROW(LS_ERR_CUDA, "the page copies failed (test hook)");
+      if (!copies.empty())
+        launch_page_copies(kc, vc, (int)c.layers, dm.kv_heads, (int)c.head_dim, pool.page(), pool.num_pages, copies.data(),
+                           copies.size(), m->num_sms, stream);
+    } catch (...) {
+      inject_err = 0;
+      pool.give_back(moves);
+      throw;
     }
-    if (!copies.empty())
-      launch_page_copies(kc, vc, (int)c.layers, dm.kv_heads, (int)c.head_dim, pool.page(), pool.num_pages, copies.data(), copies.size(),
-                         m->num_sms, stream);
+    pool.rename(moves, stream);
+    for (size_t i = 0; i < ns; i++) pool.ensure((int)(s0 + i), pos[s0 + i] + M, stream);
     const bool over_shared = plan_shared(s0, ns, M);
     std::memcpy(h_tok, tokens, T * 4);
     h2d_bytes += T * 4 + ns * 4;
@@ -2383,7 +2407,7 @@ struct LsBatch {
       LS_CUDA(cudaMemcpyAsync(h_next, d_next, nres * 4, cudaMemcpyDeviceToHost, stream));
     }
     prof_end(pp);
-    if (inject_err) {  // never captured: an injected pass runs eagerly
+    if (inject_err == 4) {  // never captured: an injected pass runs eagerly
       *h_err = inject_err;
       LS_CUDA(cudaMemcpyAsync(d_err, h_err, 4, cudaMemcpyHostToDevice, stream));
       LS_CUDA(cudaStreamSynchronize(stream));
@@ -3256,7 +3280,7 @@ int ls_model_inject_stall(LsModel* m, int barrier) {
 int ls_batch_inject_error(LsBatch* b, int code) {
   return guard([&] {
     NEED(b);
-    if (code != 0 && code != 4) LS_THROW(LS_ERR_ARG, "the injected error code must be 4 (or 0 to clear)");
+    if (code != 0 && code != 4 && code != LsBatch::kInjectCopies) LS_THROW(LS_ERR_ARG, "the injected error code must be 4 or 6 (or 0 to clear)");
     b->inject_err = code;
   });
 }

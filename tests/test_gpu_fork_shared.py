@@ -47,3 +47,23 @@ def test_the_first_shared_pass_beside_a_busy_default_stream(model):
         torch.cuda.synchronize()
         b.close()
     assert results[0] == results[1]
+
+
+def test_a_pass_that_failed_at_its_page_copies_is_made_again(model):
+    B, M, n = 5, 4, 410  # not a whole page: four of the five sequences copy the last one
+    results = []
+    for fail in (False, True):
+        b, rng = forked(model, B, M, n)
+        blocks = rng.integers(0, 150000, (4, B, M)).astype(np.uint32)
+        before = b.pages()
+        for _ in range(2 * fail):
+            b.inject_error(6)
+            with pytest.raises(ls.LayerstreamError, match="test hook") as e:
+                b.verify(blocks[0])
+            assert e.value.code == -3 and b.pages() == before and [b.pos(i) for i in range(B)] == [n] * B
+        got = [b.verify(x) for x in blocks]
+        b.fork(0, 1, n)  # the prompt's rows are still whole in the pages that are shared
+        b.truncate(0, n)
+        results.append((got, b.verify(blocks[1]), b.pages()))
+        b.close()
+    assert results[0] == results[1]
