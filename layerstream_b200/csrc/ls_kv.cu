@@ -1066,17 +1066,22 @@ void KvWork::open(const KvGeom& geom, bool is_bf16, int* err_word, cudaStream_t 
   const size_t qrows = g.rows_cap() * g.kv_heads;
   const size_t bp = up(g.plan_cap()), bq = up(qrows * g.hd * 2), bo = up(g.slots_cap() * (g.hd + 2) * 4), bf = up((size_t)g.nseq * g.kv_heads * 4);
   LS_CUDA(cudaMalloc(&mem, bp + bq + bo + bf));
-  uint8_t* p = reinterpret_cast<uint8_t*>(mem);
-  plan = p;
-  q = p + bp;
-  part = reinterpret_cast<float*>(p + bp + bq);
-  flags = reinterpret_cast<int*>(p + bp + bq + bo);
-  // the query operand's rows past the block's are read into tiles (and never used): finite from the start. In the
-  // order of the stream that uses them first: cudaMemset's is the legacy stream, which a non-blocking one passes.
-  LS_CUDA(cudaMemsetAsync(q, 0, bq, s));
-  LS_CUDA(cudaMemsetAsync(flags, 0, bf, s));
-  kv_encode_map(&qmap, q, qrows, g.hd, KV_TILE, bf16);
-  kv_encode_map(&qmap_half, q, qrows, g.hd, KV_TILE / 2, bf16);
+  try {
+    uint8_t* p = reinterpret_cast<uint8_t*>(mem);
+    plan = p;
+    q = p + bp;
+    part = reinterpret_cast<float*>(p + bp + bq);
+    flags = reinterpret_cast<int*>(p + bp + bq + bo);
+    // the query operand's rows past the block's are read into tiles (and never used): finite from the start. In the
+    // order of the stream that uses them first: cudaMemset's is the legacy stream, which a non-blocking one passes.
+    LS_CUDA(cudaMemsetAsync(q, 0, bq, s));
+    LS_CUDA(cudaMemsetAsync(flags, 0, bf, s));
+    kv_encode_map(&qmap, q, qrows, g.hd, KV_TILE, bf16);
+    kv_encode_map(&qmap_half, q, qrows, g.hd, KV_TILE / 2, bf16);
+  } catch (...) {  // (mem says whether this is open)
+    close();
+    throw;
+  }
 }
 
 void KvWork::close() {

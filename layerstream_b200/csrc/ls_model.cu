@@ -2162,7 +2162,7 @@ struct LsBatch {
       g.max_rows = (int)(B * max_block);
       g.nctas = m->num_sms;
       planner.g = g;
-      h_plan = halloc<uint8_t>(g.plan_cap());
+      if (!h_plan) h_plan = halloc<uint8_t>(g.plan_cap());  // (a pass before may have found no memory for the rest)
       kv_maps.resize(2 * c.layers);
       for (size_t l = 0; l < c.layers; l++)
         for (int i = 0; i < 2; i++)
