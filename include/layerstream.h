@@ -230,6 +230,8 @@ int ls_batch_truncate(LsBatch *b, uint64_t seq, uint64_t pos);
 int ls_batch_fork(LsBatch *b, uint64_t src, const uint64_t *dst, uint64_t ndst, uint64_t n);
 /* Pages of the batch's pool that some sequence holds, and those that more than one holds. */
 int ls_batch_pages(const LsBatch *b, uint64_t *used, uint64_t *shared);
+/* Positions that the last pass read once for several sequences (0: every sequence read its own context). */
+int ls_batch_shared_positions(const LsBatch *b, uint64_t *n);
 /* src/model.rs:111-119 for sequence `seq`: pushes n tokens, returns the greedy token after them. */
 int ls_batch_prefill(LsBatch *b, uint64_t seq, const uint32_t *ids, uint64_t n, uint32_t *argmax);
 /* ls_verify for sequences 0..nseq-1 in one pass: blocks [nseq][M]; per sequence the accepted

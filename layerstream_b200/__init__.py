@@ -114,6 +114,7 @@ _SIGS = {
     "ls_batch_truncate": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64]),
     "ls_batch_fork": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64]),
     "ls_batch_pages": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
+    "ls_batch_shared_positions": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
     "ls_batch_prefill": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.POINTER(C.c_uint32)]),
     "ls_batch_verify": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p]),
     "ls_batch_spec": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64,
@@ -355,6 +356,13 @@ class Batch:
         u, s = C.c_uint64(), C.c_uint64()
         _check(lib().ls_batch_pages(self._h, C.byref(u), C.byref(s)))
         return {"used": u.value, "shared": s.value}
+
+    @property
+    def shared_positions(self) -> int:
+        """Positions that the last pass read once for several sequences (0: every sequence read its own context)."""
+        n = C.c_uint64()
+        _check(lib().ls_batch_shared_positions(self._h, C.byref(n)))
+        return n.value
 
     def prefill(self, seq: int, ids) -> int:
         a = _u32(ids)

@@ -1615,6 +1615,7 @@ struct LsBatch {
   uint8_t* h_plan = nullptr;
   std::vector<PageCopy> copies;
   std::vector<PagePool::Move> moves;
+  size_t last_shared = 0;                      // positions that the last pass read once for several sequences
   uint32_t *h_tok = nullptr, *h_m = nullptr, *h_next = nullptr;
   int *h_pos0 = nullptr, *h_err = nullptr;
   int inject_err = 0;      // test hook: the next pass reports this error code (a host-made fault), or fails at its page copies
@@ -2219,6 +2220,7 @@ struct LsBatch {
     pool.rename(moves, stream);
     for (size_t i = 0; i < ns; i++) pool.ensure((int)(s0 + i), pos[s0 + i] + M, stream);
     const bool over_shared = plan_shared(s0, ns, M);
+    last_shared = over_shared ? planner.shared_positions() : 0;
     std::memcpy(h_tok, tokens, T * 4);
     h2d_bytes += T * 4 + ns * 4;
     const bool streamed = m->mode != LS_MODE_RESIDENT;
@@ -3208,6 +3210,14 @@ int ls_batch_pages(const LsBatch* b, uint64_t* used, uint64_t* shared) {
     NEED(b);
     if (used) *used = (uint64_t)b->pool.used();
     if (shared) *shared = (uint64_t)b->pool.nshared;
+  });
+}
+
+int ls_batch_shared_positions(const LsBatch* b, uint64_t* n) {
+  return guard([&] {
+    NEED(b);
+    NEED(n);
+    *n = b->last_shared;
   });
 }
 

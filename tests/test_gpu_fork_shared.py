@@ -67,3 +67,62 @@ def test_a_pass_that_failed_at_its_page_copies_is_made_again(model):
         results.append((got, b.verify(blocks[1]), b.pages()))
         b.close()
     assert results[0] == results[1]
+
+
+def test_blocks_of_changing_length_read_the_prefix_once(model):
+    # 32 rows of 7 heads fill tiles of their own and are planned alone, 5 rows are not
+    B, n = 4, 520
+    b, rng = forked(model, B, 32, n)
+    assert b.shared_positions == 0  # prefilled by one sequence
+    for M, shared in ((32, 0), (5, 512), (32, 0), (1, 512), (5, 512)):
+        b.verify(rng.integers(0, 150000, (B, M)).astype(np.uint32))
+        assert b.shared_positions == shared, M
+    b.close()
+
+
+def near_ties(rows):
+    top = np.partition(rows, -2, axis=1)[:, -2:]
+    return top[:, 1] - top[:, 0] <= 2e-2  # the bound of the framework's other token comparisons
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+def test_shared_and_separate_reading_decode_alike(model, monkeypatch, groups):
+    B, M, n = 6, 4, 700
+    path = synth.ensure_lsq(ROOT, "0.5b", 0, (4, 32), (4, 32), clip=True)
+    got = {}
+    for shared in ("1", "0"):
+        for graphs in ("1", "0"):
+            monkeypatch.setenv("LS_SHARED", shared)
+            monkeypatch.setenv("LS_BATCH_GRAPHS", graphs)
+            b, rng = forked(model, B, M, n, seed=5, groups=groups)
+            out = []
+            for _ in range(3):
+                blocks = rng.integers(0, 150000, (B, M)).astype(np.uint32)
+                out.append((blocks, b.verify(blocks)))
+                assert b.shared_positions == (groups * (n // 64 * 64) if shared == "1" else 0)
+                for i in range(B):
+                    b.truncate(i, n)  # every step behind the prompt alone, whatever was accepted
+            got[shared, graphs] = out
+            b.close()
+    for shared in ("1", "0"):
+        for (_, x), (_, y) in zip(got[shared, "1"], got[shared, "0"]):
+            assert x == y  # a graph's replay is the eager pass
+    alone = ls.Model(path, max_ctx=n + 64)
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, 150000, n).tolist() for _ in range(groups)]
+    same = 0
+    for g in range(groups):
+        alone.truncate(0)
+        alone.forward(prompts[g], want_logits=False)
+        for (blocks, (m1, t1)), (_, (m0, t0)) in zip(got["1", "1"], got["0", "1"]):
+            for i in range(g * B // groups, (g + 1) * B // groups):
+                alone.truncate(n)
+                rows = alone.forward_multi(blocks[i], M)
+                k = 0
+                while k < M - 1 and rows[k].argmax() == blocks[i, k + 1]:
+                    k += 1
+                if not near_ties(rows[: k + 1]).any():
+                    same += 1
+                    assert (m1[i], t1[i]) == (m0[i], t0[i]) == (k, int(rows[k].argmax())), i
+    assert same >= 2 * B
+    alone.close()
