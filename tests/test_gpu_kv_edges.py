@@ -103,3 +103,32 @@ def test_a_begin_that_failed_is_made_again_with_its_copies():
     for layer in (0, 1):
         run_layer(s, layer, [3, 1, 2, 3])
     s.kv.end()
+
+
+@pytest.mark.parametrize("heads,kvh,hd,dtype,M", [(14, 2, 64, "f16", 1), (16, 2, 128, "bf16", 5), (8, 2, 128, "f16", 9), (6, 2, 64, "bf16", 3)])
+def test_prompts_under_a_system_prompt_are_two_shared_levels(heads, kvh, hd, dtype, M):
+    # 512 positions of all nine sequences, then 640 and 768 of four each; the ninth has only the first range
+    s = Setup(heads, kvh, hd, dtype, 64, 9, M, 1600, seed=23)
+    s.fill_fast(0, list(range(22)), 512 + 640 + 70)
+    s.fill_fast(4, list(range(8)) + list(range(30, 45)), 512 + 768 + 5)
+    s.fill_fast(8, list(range(8)) + [60, 61], 512 + 33)
+    s.kv.fork(0, [1, 2, 3], 512 + 640 + 9)
+    s.kv.fork(4, [5, 6, 7])
+    for counts in ([M] * 9, [M, 0, 1, M, 0, M, M, 1, M], [M] * 9):
+        s.kv.begin(counts, M)
+        s.kv.self_check()
+        assert s.kv.info.shared_positions == 512 + 640 + 768
+        run_layer(s, 0, counts)
+        s.kv.end()
+
+
+def test_more_segments_than_a_lane_keeps_near():
+    # 700 sequences x 16 kv heads, each with a tile of its own: 11200 segments on the 296 lanes of 148 SMs, more than 32
+    # on some lane whatever the split
+    s = Setup(16, 16, 64, "f16", 16, 700, 1, 64, seed=29, num_pages=2810)
+    for i in range(700):
+        s.fill_fast(i, [0, 1, 2 + 4 * i, 3 + 4 * i], 32 + i % 31)
+    s.kv.begin([1] * 700, 1)
+    s.kv.self_check()
+    assert s.kv.info.shared_positions == 32
+    run_layer(s, 0, [1] * 700)
