@@ -114,7 +114,7 @@ class KvPlanner {
   // version: changes whenever a page table changed other than by growing at its end (the sharing
   // tree of the last plan is kept while version and every sequence's class, by its rows, stay the same).
   void build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version);
-  // Throws unless the plan covers every row's positions exactly once and stays inside its bounds.
+  // Throws unless the plan covers every row's positions exactly once, stays inside its bounds and loads the CTAs evenly.
   void check(const std::vector<KvSeqIn>& seqs) const;
   size_t shared_positions() const { return shared_pos_; }  // positions read for several sequences at once
 
@@ -128,6 +128,7 @@ class KvPlanner {
   struct Job {
     int node, g, tile, ntiles, nch, p1;
   };
+  static double start_of(const Job& j), chunk_of(const Job& j);  // costs (ls_kv_plan.cpp)
   struct Piece {
     int cta, job, c0, nch;
   };

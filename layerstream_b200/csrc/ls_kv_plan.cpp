@@ -16,11 +16,15 @@ constexpr long long kMinSaved = 256;
 
 // Time of a CTA's work in units of one pair chunk: a chunk for two tiles, for one tile (the two lanes work on
 // different ones), and what a piece costs before its first chunk and after its last. From timelines of the CTAs
-// (hd 64 and 128, 2 to 64 readers of 2k to 64k positions): a pair chunk takes about 3400 cycles. With the starts of
-// pieces that a CTA's end cuts left out, the CTAs of single tiles ended 40 % after those of pairs; with these
+// (hd 64 and 128, 2 to 64 readers of 2k to 64k positions): a pair chunk takes about 3400 cycles. Without the starts
+// of pieces that a CTA's end cuts, the CTAs of single tiles ended 40 % after those of pairs; with them
 // all end within 15 % of the mean (four prompts of 8k with 16 samples each 61.8 against 54.8 us, a prefill of
 // eight chunks 52.8 against 46.5). A single chunk at 0.55 instead: 64 readers of 32k 68.6 against 65.4 us.
+// Dealt by shares of what is left instead of by the least time that is enough, the last CTA was left with whatever
+// the estimate of the cuts had missed: 8 sequences x 5 rows under 8192 (14/2 heads x 64) 71.5 against 13.3 us, 32 x 1
+// 36.2 against 13.2, 4 x 12 (16/2 x 128) 101 against 17.5; at most 7 % faster (4 x 48, 26.1 against 27.9).
 constexpr double kPairChunk = 1.0, kSingleChunk = 0.62, kPairStart = 1.5, kSingleStart = 0.4;
+constexpr double kDealSlack = 2 * kPairStart + kPairChunk;
 
 // A row with more partials than this is merged by a whole block instead of hd / 4 of its threads when rows and
 // heads are few (KV_SPLIT_ITEMS). 16 rows of 14 heads, 40 partials: hd / 4 threads 10.4 us, a block 5.0; 288
@@ -104,6 +108,9 @@ KvPlanner::Class KvPlanner::class_of(int cnt) const {
   return rows * 5 >= pairs * 2 * KV_TILE * 4 ? ALONE : GROUPED;
 }
 
+double KvPlanner::start_of(const Job& j) { return j.ntiles == 2 ? kPairStart : kSingleStart; }
+double KvPlanner::chunk_of(const Job& j) { return j.ntiles == 2 ? kPairChunk : kSingleChunk; }
+
 void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version) {
   std::vector<Class> now(seqs.size());
   for (size_t i = 0; i < seqs.size(); i++) now[i] = class_of(seqs[i].cnt);
@@ -186,39 +193,43 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
         }
       }
     }
-  // The jobs' chunks in order, dealt to the CTAs: each takes, to the nearest chunk, its share of what is left.
-  // Every piece pays a start, so the pieces that the CTAs' ends add are counted in before.
-  double rest = 0, pairs = 0;
-  for (const Job& j : jobs_)
-    if (j.ntiles == 2)
-      pairs += kPairStart + j.nch * kPairChunk;
-    else
-      rest += kSingleStart + j.nch * kSingleChunk;
-  rest += pairs;
-  if (rest > 0) rest += g.nctas * (kPairStart * pairs + kSingleStart * (rest - pairs)) / rest;
-  pieces_.clear();
-  {
+  // The jobs' chunks in order, dealt to the CTAs: each takes what fits into its time, at least one chunk; the least time
+  // for which the CTAs are enough is searched for, to 2 %. A CTA wastes less than a start and a chunk and pays one
+  // start that a cut added, so kDealSlack above the mean is always enough.
+  double work = 0, least = 0;
+  for (const Job& j : jobs_) {
+    work += start_of(j) + j.nch * chunk_of(j);
+    least = std::max(least, start_of(j) + chunk_of(j));
+  }
+  auto deal = [&](double time, bool keep) {  // CTAs that it takes
     int cta = 0;
-    double room = rest / g.nctas;
+    double room = time;
     for (size_t k = 0; k < jobs_.size(); k++) {
-      const bool pair = jobs_[k].ntiles == 2;
-      const double q = pair ? kPairChunk : kSingleChunk, o = pair ? kPairStart : kSingleStart;
+      const double q = chunk_of(jobs_[k]), o = start_of(jobs_[k]);
       for (int c = 0; c < jobs_[k].nch;) {
-        int take = jobs_[k].nch - c;
-        if (cta < g.nctas - 1) {
-          const int fit = (int)((room - o) / q + 0.5);
-          if (fit < 1) {
-            room = rest / (g.nctas - ++cta);
-            if (room >= o + 0.5 * q) continue;
-          }
-          take = std::min(take, std::max(fit, 1));
+        const double fit = (room - o) / q;
+        if (fit < 1) {  // (never in a CTA that has nothing yet)
+          cta++;
+          room = time;
+          continue;
         }
-        pieces_.push_back({cta, (int)k, c, take});
+        const int take = fit < jobs_[k].nch - c ? (int)fit : jobs_[k].nch - c;
+        if (keep) pieces_.push_back({cta, (int)k, c, take});
         room -= o + take * q;
-        rest -= o + take * q;
         c += take;
       }
     }
+    return cta + 1;
+  };
+  pieces_.clear();
+  if (!jobs_.empty()) {
+    double low = std::max(work / g.nctas, least * (1 + 1e-9)), high = low + kDealSlack;
+    if (deal(low, false) <= g.nctas) high = low;
+    while (high - low > 0.02 * low) {
+      const double mid = (low + high) / 2;
+      (deal(mid, false) <= g.nctas ? high : low) = mid;
+    }
+    deal(high, true);
   }
   // segments
   segs_.clear();
@@ -320,7 +331,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   if (at > g.plan_cap()) LS_THROW(LS_ERR_ARG, "internal: an attention plan outgrew its workspace");
 }
 
-// Reads the packed plan as the kernels do.
+// Reads the packed plan as the kernels do (the jobs' costs are the last build's).
 void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
   auto need = [](bool ok, const char* what) {
     if (!ok) LS_THROW(LS_ERR_ARG, std::string("attention plan: ") + what);
@@ -337,6 +348,12 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
   std::unordered_map<int, const KvSeg*> at;
   size_t nseg = 0;
   std::vector<uint8_t> written(h.nslots, 0);
+  double work = 0, least = 0;
+  for (const Job& j : jobs_) {
+    work += start_of(j) + j.nch * chunk_of(j);
+    least = std::max(least, start_of(j) + chunk_of(j));
+  }
+  const double longest = std::max(work / g.nctas, least) + kDealSlack;
   for (int c = 0; c < g.nctas; c++) {
     const KvProg& p = prog[c];
     int pair_ch = 0, own[2] = {0, 0};
@@ -373,6 +390,7 @@ void KvPlanner::check(const std::vector<KvSeqIn>& seqs) const {
       }
     }
     need(pair_ch == p.pair_ch && (own[0] == own[1] || own[0] == own[1] + 1), "lane balance");
+    need(p.npair * kPairStart + pair_ch * kPairChunk + (own[0] + own[1]) * kSingleChunk <= longest, "a CTA's share of the work");
   }
   need(nseg == at.size(), "segments");
   // every row's path: positions covered once, through pages equal to its own

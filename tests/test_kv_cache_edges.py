@@ -92,3 +92,17 @@ def test_a_begin_that_fails_changes_nothing(seed):
     a.begin([0] * 5, 1)
     for code in (-1, 2, 3):
         refuses(a.inject_error, code)
+
+
+@pytest.mark.parametrize("heads,hd", [(14, 64), (16, 128), (6, 64)])
+@pytest.mark.parametrize("prefix", [512, 2048, 8192, 32768])
+def test_no_cta_gets_the_rest_of_the_work(heads, hd, prefix):
+    # (self_check compares every CTA's share with the mean) shared tiles in pairs and single ones, long and short ranges
+    for seqs in (1, 2, 4, 8, 32):
+        for M in (1, 3, 5, 9, 12, 16, 20, 33, 40, 48, 64):
+            kv = cache(seqs=seqs, page=64, num_pages=prefix // 64 + 3 * seqs, max_ctx=prefix + 192, max_rows=seqs * M, heads=heads, hd=hd)
+            for s in range(seqs):
+                kv.set_table(s, [*range(prefix // 64), *range(prefix // 64 + 3 * s, prefix // 64 + 3 * s + 3)], prefix + 100)
+            kv.begin([M] * seqs, M)
+            kv.self_check()
+            kv.close()
