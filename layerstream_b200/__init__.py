@@ -191,6 +191,14 @@ def _ints(a):
     return a.tolist() if isinstance(a, np.ndarray) else a
 
 
+def _seqs(dst) -> array:
+    """One sequence number (any integer type) or several."""
+    try:
+        return array("Q", [dst] if isinstance(dst, (int, np.integer)) else dst)
+    except OverflowError as e:
+        raise ValueError("sequence numbers must be in 0..2^64-1") from e
+
+
 def _addr(a: np.ndarray) -> int:
     """The array's address, without _p's cost (4 us); the caller keeps the array."""
     return a.__array_interface__["data"][0]
@@ -349,7 +357,7 @@ class Batch:
     def fork(self, src: int, dst, n: int | None = None):
         """dst (one sequence or several) hold the first n positions of src (None: all), in the same K/V pages;
         verify passes then read the shared prefix once for all of its sequences."""
-        d = array("Q", [dst] if isinstance(dst, int) else dst)
+        d = _seqs(dst)
         _check(lib().ls_batch_fork(self._h, src, d.buffer_info()[0], len(d), self.pos(src) if n is None else n))
 
     def pages(self) -> dict:
@@ -634,7 +642,7 @@ class KvCache:
 
     def fork(self, src: int, dst, n: int | None = None):
         """dst (one sequence or several) hold the first n positions of src (None: all), in the same pages."""
-        d = array("Q", [dst] if isinstance(dst, int) else dst)
+        d = _seqs(dst)
         _check(lib().ls_kv_fork(self._h, src, d.buffer_info()[0], len(d), self.length(src) if n is None else n))
 
     def truncate(self, seq: int, n: int):

@@ -106,3 +106,19 @@ def test_no_cta_gets_the_rest_of_the_work(heads, hd, prefix):
             kv.begin([M] * seqs, M)
             kv.self_check()
             kv.close()
+
+
+def test_fork_takes_any_integer_and_any_sequence_of_them():
+    kv = cache(seqs=6)
+    kv.begin([5, 0, 0, 0, 0, 0], 5)
+    kv.end()
+    for dst in (np.int64(1), np.uint32(2), [np.int32(3)], (5,), np.array([1, 2]), range(3, 5)):
+        kv.fork(0, dst)
+    assert [kv.length(s) for s in range(6)] == [5] * 6
+    for dst in (-1, [1, -2], np.int64(-1)):
+        with pytest.raises(ValueError):
+            kv.fork(0, dst)
+    for dst in (1.0, [1.5], "12"):
+        with pytest.raises(TypeError):
+            kv.fork(0, dst)
+    kv.self_check()
