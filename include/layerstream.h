@@ -327,8 +327,12 @@ int ls_kv_begin(LsKv *kv, const uint32_t *counts, uint64_t M, void *stream);
  * they are rotated already. k and v are rounded into the sequence's pages at position len + t; the row
  * attends to positions 0 .. len + t. Rows t >= counts[s] are neither read nor written. Scores, softmax
  * statistics and sums are f32; q (rotated) and the softmax weights are rounded to the cache's type for
- * the tensor cores. Device pointers, 16-byte aligned; strides multiples of 8. An error that the kernels
- * report (LS_ERR_DEVICE) comes with the next call. */
+ * the tensor cores. Device pointers, 16-byte aligned; strides multiples of 8.
+ *
+ * A kernel whose bounded wait runs out returns and leaves the GPU usable; the next ls_kv_begin, ls_kv_attention
+ * or ls_kv_compact then fails with LS_ERR_DEVICE, and so does every later one: the outputs since the last call that
+ * was waited for are not to be trusted, nor are rows that were kept since. The lengths and tables can still be
+ * read and truncated, and a new cache over the same pools goes on from them (ls_kv_open, ls_kv_set). */
 int ls_kv_attention(LsKv *kv, uint64_t layer, const void *qkv, uint64_t qkv_stride, const float *rope, void *out,
                     uint64_t out_stride, void *stream);
 int ls_kv_end(LsKv *kv, const uint32_t *keep);

@@ -132,3 +132,32 @@ def test_more_segments_than_a_lane_keeps_near():
     s.kv.self_check()
     assert s.kv.info.shared_positions == 32
     run_layer(s, 0, [1] * 700)
+
+
+def test_after_a_wait_ran_out_a_new_cache_goes_on_over_the_same_pools():
+    args = (4, 2, 64, "f16", 16, 3, 2, 400)
+    s = Setup(*args, seed=31)
+    s.fill_fast(0, list(range(20)), 300)
+    s.kv.fork(0, [1, 2])
+    s.kv.begin([2, 1, 2], 2)
+    run_layer(s, 0, [2, 1, 2])
+    s.kv.end()
+    s.kv.begin([1, 1, 1], 2)
+    s.kv.inject_error(2)
+    x = s.randn(6, s.W)
+    for _ in range(2):
+        for call in (lambda: s.kv.begin([1, 1, 1], 2), lambda: s.kv.attention(0, x.data_ptr(), x.data_ptr()), s.kv.compact):
+            with pytest.raises(ls.LayerstreamError, match="bounded wait") as e:
+                call()
+            assert e.value.code == -4
+    s.kv.truncate(1, 300)
+    lens, tables = [s.kv.length(i) for i in range(3)], s.kv.tables()
+    assert lens == [302, 300, 302]
+    s.kv.close()
+    s.kv = ls.KvCache(s.k.data_ptr(), s.v.data_ptr(), layers=1, heads=4, kv_heads=2, hd=64, page=16, num_pages=s.num_pages, seqs=3,
+                      max_ctx=400, max_rows=6, dtype="f16")
+    for i, n in enumerate(lens):
+        s.kv.set_table(i, tables[i][: -(-n // 16)], n)
+    s.kv.begin([2, 2, 0], 2)
+    s.kv.self_check()
+    run_layer(s, 0, [2, 2, 0])
