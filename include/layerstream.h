@@ -225,7 +225,7 @@ int ls_batch_truncate(LsBatch *b, uint64_t seq, uint64_t pos);
  * position) in the same K/V pages, and nothing else (best-of-n sampling, many questions about one
  * prompt: prefilled once). A page is copied when one of several holders is about to write into it, and a
  * verify pass reads a prefix that several of its sequences share once for all of them (f16 cache, head
- * sizes 64 and 128; other shapes read it per sequence). On a tensor-parallel batch every rank makes
+ * sizes 64 and 128; other shapes read it per sequence, and so do blocks whose rows fill 128-row tiles by themselves). On a tensor-parallel batch every rank makes
  * the call. */
 int ls_batch_fork(LsBatch *b, uint64_t src, const uint64_t *dst, uint64_t ndst, uint64_t n);
 /* Pages of the batch's pool that some sequence holds, and those that more than one holds. */
@@ -276,8 +276,9 @@ int ls_batch_tp_peer(const LsBatch *b, int *on);
  *
  * Pools: k_pool, v_pool [layers][kv_heads][num_pages][page][hd], 16-bit (dtype), 16-byte aligned, on
  * `device`; rows past a sequence's length are never used. page: a power of two in 8..65536; hd: 64 or
- * 128. max_ctx: positions of one sequence; max_rows: largest seqs x M of a step (sizes the workspaces,
- * which the cache owns and allocates here). device -1: the bookkeeping alone, without a GPU (pools
+ * 128. max_ctx: positions of one sequence; max_rows: largest seqs x M of a step. It sizes the workspaces,
+ * which the cache owns and allocates here: about 14 hd + 24 bytes for every head of every row (0.47 GB for 8192
+ * rows of 32 heads of 128) and 15 to 30 MB. device -1: the bookkeeping alone, without a GPU (pools
  * NULL; attention is refused).
  *
  * A step, per decode or verify pass: ls_kv_begin gives every sequence s counts[s] (0..M) rows behind
@@ -327,7 +328,8 @@ int ls_kv_begin(LsKv *kv, const uint32_t *counts, uint64_t M, void *stream);
  * they are rotated already. k and v are rounded into the sequence's pages at position len + t; the row
  * attends to positions 0 .. len + t. Rows t >= counts[s] are neither read nor written. Scores, softmax
  * statistics and sums are f32; q (rotated) and the softmax weights are rounded to the cache's type for
- * the tensor cores. Device pointers, 16-byte aligned; strides multiples of 8.
+ * the tensor cores. Weights reach 2^8 before they are divided by their sum, so sums with V of 2^119 and more (bf16)
+ * may overflow for the rows that see it. Device pointers, 16-byte aligned; strides multiples of 8.
  *
  * A kernel whose bounded wait runs out returns and leaves the GPU usable; the next ls_kv_begin, ls_kv_attention
  * or ls_kv_compact then fails with LS_ERR_DEVICE, and so does every later one: the outputs since the last call that

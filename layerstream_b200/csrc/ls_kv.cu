@@ -17,9 +17,10 @@
 // Warp roles of kv_attn_kernel: two softmax warpgroups (one per lane of the CTA), one MMA issuer warp
 // per lane, one TMA producer warp. K and V come in chunks of 128 positions; the softmax takes them by halves of
 // 64, so that a lane's two S buffers fit beside O in tensor memory at hd 128 too, and the tensor cores work
-// on one half while the softmax works on the other. (One buffer of 128 positions: 107 instead of 90 us
-// for many pair tiles at hd 128; at hd 64, where the next S could follow as soon as the last one was in
-// registers, 75 us either way.) O stays in tensor memory and is rescaled only when a row's maximum has
+// on one half while the softmax works on the other. (Many pair tiles: 64 sequences of 32 rows, 4096 positions
+// each, 16/2 heads of 128 in bf16 or 14/2 of 64 in f16, one call in a graph. One buffer of 128 positions: 107 instead
+// of 90 us at hd 128; at hd 64, where the next S could follow as soon as the last one was in registers, 75 us
+// either way.) O stays in tensor memory and is rescaled only when a row's maximum has
 // grown by more than 2^8 over the one its exponents are taken against.
 //
 // Bound, per two tiles and 128 positions: the special-function units need 2048 clocks for the exponentials

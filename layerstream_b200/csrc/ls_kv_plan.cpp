@@ -11,7 +11,11 @@ namespace ls {
 
 // A range is read for its sequences at once when that saves at least this many position reads over
 // the sequences reading it one by one: below it, the extra partial that every row then leaves and
-// joins costs about as much as the reads.
+// joins costs about as much as the reads. Calls in a graph, single rows of 2 to 64 sequences, 14/2 heads of 64, 16/2
+// and 32/8 of 128, read at once against one by one: 3 to 7 % slower where 32 to 200 reads are saved (two
+// sequences under 64 positions 7.66 against 7.31 us), within 4 % either way from 256 to 1500, then up to 8 % faster with
+// 2 kv heads (64 under 512: 10.4 against 11.3) and up to 51 % with 8 (14.5 against 29.6). It stays slower, by up to
+// 13 %, for 16 to 64 sequences under at most 256 positions at hd 128 with 2 kv heads (64 under 128: 11.8 against 10.4).
 constexpr long long kMinSaved = 256;
 
 // Time of a CTA's work in units of one pair chunk: a chunk for two tiles, for one tile (the two lanes work on
@@ -104,6 +108,9 @@ KvPlanner::Class KvPlanner::class_of(int cnt) const {
   if (cnt == 0) return IDLE;
   // rows that fill tiles of their own read the prefix once per pair of tiles either way: as one range with
   // their own positions they leave one partial less
+  // (2 to 8 sequences of 16 to 128 rows under 1k to 8k: blocks that fill their pairs to 0.9 and more take up to 31 %
+  // longer in a group, 8 x 128 rows of 16/2 heads of 128 under 8k 100.9 against 77.1 us; blocks that fill them to 0.5 to
+  // 0.7 take up to 16 % longer alone, 8 x 20 rows of 14/2 heads of 64 under 8k 24.2 against 20.4)
   const int rows = cnt * g.G(), pairs = (rows + 2 * KV_TILE - 1) / (2 * KV_TILE);
   return rows * 5 >= pairs * 2 * KV_TILE * 4 ? ALONE : GROUPED;
 }
