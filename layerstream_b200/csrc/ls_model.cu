@@ -2145,7 +2145,7 @@ struct LsBatch {
 
   // Whether the pass of sequences s0 .. s0 + ns - 1, M rows each, reads a prefix that several of them hold in the
   // same pages; its plan is then on the device. LS_SHARED=0: every sequence reads its own context.
-  // The whole pass goes that way as soon as one range is shared: it was faster in all 31 shapes measured, also where 2 of
+  // The whole pass goes that way as soon as one range is shared: it was faster in all 33 shapes measured, also where 2 of
   // 32 sequences share 256 positions (0.5B, separate against shared: 1.80 and 1.61 ms at M = 1, 4.39 and 4.04 at M = 9;
   // two layers of the 3B shape 1.20 and 1.16), by 3 to 47 % over 2 to 32 sequences, 300 to 8000 positions, M = 1 to 33.
   bool plan_shared(size_t s0, size_t ns, int M) {
