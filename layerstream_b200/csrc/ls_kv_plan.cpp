@@ -123,6 +123,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
   for (size_t i = 0; i < seqs.size(); i++) now[i] = class_of(seqs[i].cnt);
   if (version != version_ || now != class_) {
     class_ = now;
+    version_ = ~0ull;  // (kept if tree throws: the next build makes it anew)
     tree(seqs);
     version_ = version;
   }
@@ -236,7 +237,7 @@ void KvPlanner::build(const std::vector<KvSeqIn>& seqs, int M, uint64_t version)
       const double mid = (low + high) / 2;
       (deal(mid, false) <= g.nctas ? high : low) = mid;
     }
-    deal(high, true);
+    if (deal(high, true) > g.nctas) LS_THROW(LS_ERR_ARG, "internal: an attention plan needs more CTAs than there are");
   }
   // segments
   segs_.clear();
