@@ -186,9 +186,9 @@ def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
 
-def _ints(a):
-    """Arrays as lists: np.array(list, np.int32) refuses what does not fit, a cast of an array would wrap."""
-    return a.tolist() if isinstance(a, np.ndarray) else a
+def _ints(a) -> array:
+    """32-bit integers; what does not fit and what is no integer is refused (a cast would wrap or cut it)."""
+    return array("i", a.tolist() if isinstance(a, np.ndarray) else a)
 
 
 def _seqs(dst) -> array:
@@ -637,8 +637,8 @@ class KvCache:
 
     def set_table(self, seq: int, pages, n: int):
         """Sequence seq holds exactly these pages, n positions of them cached."""
-        p = np.array(_ints(pages), np.int32)
-        _check(lib().ls_kv_set(self._h, seq, _addr(p), p.size, n))
+        p = _ints(pages)
+        _check(lib().ls_kv_set(self._h, seq, p.buffer_info()[0], len(p), n))
 
     def fork(self, src: int, dst, n: int | None = None):
         """dst (one sequence or several) hold the first n positions of src (None: all), in the same pages."""
@@ -700,16 +700,12 @@ class KvCache:
 def kv_copy_pages(k_ptr: int, v_ptr: int, layers: int, kv_heads: int, hd: int, page: int, num_pages: int, src, dst, rows=None,
                   stream: int = 0):
     """Rows [0, rows[i]) (None: whole pages) of page src[i] to page dst[i], in every layer and kv head of both pools."""
-    lists = [_ints(a) for a in ((src, dst) if rows is None else (src, dst, rows))]
-    try:
-        lists = np.array(lists, np.int32)  # (one array: small calls are host-bound)
-    except ValueError:
-        lists = None
-    if lists is None or lists.ndim != 2:
+    src, dst, rows = _ints(src), _ints(dst), None if rows is None else _ints(rows)
+    n = len(src)
+    if len(dst) != n or (rows is not None and len(rows) != n):
         raise ValueError("src, dst and rows must have the same length")
-    n, at = lists.shape[1], _addr(lists)
-    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, at, at + 4 * n, None if rows is None else at + 8 * n,
-                                  n, stream))
+    _check(lib().ls_kv_copy_pages(k_ptr, v_ptr, layers, kv_heads, hd, page, num_pages, src.buffer_info()[0], dst.buffer_info()[0],
+                                  None if rows is None else rows.buffer_info()[0], n, stream))
 
 
 def qgemv_rows_noalloc(bits: int, group: int, rows_ptr: int, rows: int, cols: int, x_ptr: int, M: int, y_ptr: int,

@@ -122,3 +122,21 @@ def test_fork_takes_any_integer_and_any_sequence_of_them():
         with pytest.raises(TypeError):
             kv.fork(0, dst)
     kv.self_check()
+
+
+def test_pages_that_are_no_integers_are_refused():
+    kv = cache()
+    kv.set_table(1, [3, np.int64(4)], 9)
+    before = kv.tables()
+    for ids in ([0.5], [1.0], np.array([1.5, 2.5]), ["1"], [None]):
+        with pytest.raises(TypeError):
+            kv.set_table(0, ids, 0)
+        with pytest.raises(TypeError):
+            ls.kv_copy_pages(1 << 20, 1 << 20, 1, 1, 64, 16, 8, ids, list(range(len(ids))))
+        with pytest.raises(TypeError):
+            ls.kv_copy_pages(1 << 20, 1 << 20, 1, 1, 64, 16, 8, list(range(len(ids))), list(range(4, 4 + len(ids))), ids)
+    for ids in ((5, 6), range(5, 7), np.array([5, 6], np.uint8), [np.int32(5), 6]):
+        kv.set_table(0, ids, 9)
+        assert kv.tables()[0, :3].tolist() == [5, 6, -1]
+    assert np.array_equal(kv.tables()[1], before[1])
+    ls.kv_copy_pages(1 << 20, 1 << 20, 1, 1, 64, 16, 8, [], [], [])
