@@ -161,3 +161,90 @@ def test_after_a_wait_ran_out_a_new_cache_goes_on_over_the_same_pools():
     s.kv.begin([2, 2, 0], 2)
     s.kv.self_check()
     run_layer(s, 0, [2, 2, 0])
+
+
+@pytest.mark.parametrize("heads,kvh,hd,dtype,page,n,M", [
+    (14, 2, 64, "f16", 64, 70, 1500),      # a long block: 83 tiles of one sequence, rows that see chunks of new rows alone
+    (8, 1, 128, "bf16", 128, 1000, 700),
+    (128, 1, 64, "f16", 16, 200, 3),       # a row's heads fill a tile, or more than one
+    (200, 1, 128, "bf16", 32, 300, 2),
+    (1024, 8, 64, "bf16", 64, 40, 1),
+    (4, 1, 64, "f16", 65536, 3000, 2),     # the largest page
+    (3, 3, 128, "bf16", 2048, 2047, 3),    # rows on both sides of a page's end
+])
+def test_sizes_at_the_ends_of_the_range(heads, kvh, hd, dtype, page, n, M):
+    s = Setup(heads, kvh, hd, dtype, page, 2, M, n + M, seed=37)
+    s.fill_fast(0, list(range(-(-n // page))), n)
+    s.kv.fork(0, [1], n - n % 16)
+    counts = [M, max(1, M // 3)]
+    s.kv.begin(counts, M)
+    s.kv.self_check()
+    run_layer(s, 0, counts)
+
+
+def test_pools_of_more_than_2_to_the_31_elements():
+    # 19.2 million rows of 128: pages at both ends of the pools, in the second layer's half of them; copied pages too
+    s = Setup(4, 1, 128, "f16", 64, 3, 2, 700, layers=2, seed=41, num_pages=150000)
+    ids = [149999, 0, 149990, 75000, 149998, 1, 149997, 149996, 2, 149995]
+    s.fill_fast(0, ids, 620)
+    s.kv.fork(0, [1, 2], 600)
+    s.kv.begin([2, 2, 1], 2)
+    s.kv.self_check()
+    assert s.kv.info.shared_positions == 576
+    run_layer(s, 1, [2, 2, 1])
+    s.kv.end()
+    t, lens = s.kv.tables(), [s.kv.length(i) for i in range(3)]
+    assert lens == [622, 602, 601]
+    old = [s.k[:, :, t[i, : -(-lens[i] // 64)].tolist()].clone() for i in range(3)]
+    moved = s.kv.compact()
+    torch.cuda.synchronize()
+    t = s.kv.tables()
+    assert moved > 5 and t.max() == s.kv.info.pages_used - 1
+    for i in range(3):
+        new = s.k[:, :, t[i, : -(-lens[i] // 64)].tolist()]
+        assert torch.equal(new.view(torch.int16), old[i].view(torch.int16))
+    s.kv.begin([1, 1, 1], 2)
+    run_layer(s, 1, [1, 1, 1])
+
+
+def test_a_step_begun_on_one_stream_and_read_on_another():
+    s = Setup(8, 2, 64, "f16", 32, 4, 2, 900, layers=2, seed=43)
+    s.fill_fast(0, list(range(25)), 790)
+    s.kv.fork(0, [1, 2, 3])
+    qkv, outs = s.randn(8, s.W), []
+    torch.cuda.synchronize()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    for a, b in ((first, second), (second, first)) * 5:
+        s.kv.begin([2, 2, 1, 2], 2, a.cuda_stream)
+        b.wait_stream(a)
+        out = torch.zeros(8, 8 * 64, device="cuda", dtype=s.dt)
+        b.wait_stream(torch.cuda.current_stream())
+        s.kv.attention(1, qkv.data_ptr(), out.data_ptr(), s.rope.data_ptr(), stream=b.cuda_stream)
+        a.wait_stream(b)
+        outs.append(out)  # the step is dropped: every turn begins the same one again
+    torch.cuda.synchronize()
+    s.kv.begin([2, 2, 1, 2], 2)
+    want = run_layer(s, 1, [2, 2, 1, 2], qkv)
+    rows = [0, 1, 2, 3, 4, 6, 7]
+    for out in outs:
+        assert torch.equal(out[rows], want[rows])
+
+
+def test_page_copies_in_a_captured_graph():
+    k, v = (torch.randn(2, 2, 12, 16, 64, device="cuda").half() for _ in range(2))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        ls.kv_copy_pages(k.data_ptr(), v.data_ptr(), 2, 2, 64, 16, 12, [0, 0, 3], [5, 6, 7], [16, 16, 3], st.cuda_stream)
+    for _ in range(2):
+        k.copy_(torch.randn(k.shape, device="cuda"))
+        v.copy_(torch.randn(v.shape, device="cuda"))
+        want = [x.clone() for x in (k, v)]
+        for w in want:
+            w[:, :, 5] = w[:, :, 6] = w[:, :, 0]
+            w[:, :, 7, :3] = w[:, :, 3, :3]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
